@@ -348,6 +348,103 @@ int vx_tp_p2p_open(vx_handle* h, const uint8_t* handles /* [tp_size][64] */);
 int vx_lm_head_argmax_noalloc(const uint16_t* weight, const float* x, int32_t rows, int32_t dim, int32_t* out_index,
                               float* out_value, void* stream, char* err, size_t err_len);
 
+/* ---- Serving operators on the caller's device memory.  Like vx_lm_head_argmax_noalloc they
+ * need no handle and allocate nothing: every pointer is device memory of the current device
+ * unless a comment says otherwise, work is enqueued on `stream` (cudaStream_t, NULL = default
+ * stream) and the call returns without waiting.  They may be captured into a CUDA graph; calls
+ * on several streams may overlap as long as they share no output and no workspace.  err
+ * (nullable) receives a message.  No counterpart in the reference, which decodes one utterance
+ * with an f32 cache (src/engine.ts:814-1042).
+ * Element types: 0 F16, 1 BF16, 2 F32 (as in vx_load_tensor_typed).  Strides count elements; the
+ * innermost dimension is contiguous; rows start on 16-byte boundaries.
+ * status (nullable, int32, set to 0 by the caller): keeps the first VX_STATUS_* a kernel met. */
+#define VX_STATUS_WAIT_1 1    /* a bounded wait of a kernel expired (codes 1 to 4 and 6)       */
+#define VX_STATUS_BAD_INDEX 5 /* a page, sequence, offset or length out of range: such a token is
+                                 not written, keys of such a page read as zero                 */
+
+/* One layer of a paged K/V cache: element (page, head, slot, d) of each pool at
+ * page * page_stride + head * head_stride + slot * slot_stride + d.  The engine's own layout
+ * ([page][layer][K|V][head][64][128]) is such a pool, and so is a token-major one. */
+typedef struct vx_kv_pages {
+  void *k, *v;
+  int64_t k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_page_stride, v_head_stride, v_slot_stride;
+  int32_t n_pages, n_kv_heads, page_size, head_dim;
+  int32_t dtype, reserved; /* F16 or BF16 */
+} vx_kv_pages;
+
+/* Rotary positions and the cache append of a ragged batch.  Token t of sequence seq_ids[t] at
+ * position positions[t]: q (n_heads rows; n_heads 0: none) rotated into q_out in the cache's type,
+ * k rotated and v unchanged written to slot position % page_size of page
+ * page_table[seq * table_stride + position / page_size].  Pair i turns by position * rope_freq[i]
+ * (formed in f64): elements (2i, 2i+1) if interleaved, else (i, i + rot_dim / 2); elements from
+ * rot_dim on pass through.  A negative position is padding: nothing of that token is written.
+ * Two tokens for one slot leave either (or a mixture).  q_out may be q itself where the
+ * types are the same.  head_dim and rot_dim: multiples of 16, at most 512. */
+typedef struct vx_rope_append_args {
+  vx_kv_pages cache;
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride;
+  const int32_t *page_table, *seq_ids, *positions;
+  const float* rope_freq; /* [rot_dim / 2] */
+  int32_t* status;
+  int64_t table_stride;
+  int32_t dtype; /* of q, k and v */
+  int32_t n_tokens, n_heads, n_seqs, max_pages, rot_dim, interleaved, reserved;
+} vx_rope_append_args;
+int vx_rope_append_kv(const vx_rope_append_args* a, void* stream, char* err, size_t err_len);
+
+/* Attention of a batch whose sequences share a prefix.  Sequence b holds the prefix_len keys in
+ * prefix_pages (shared by all) and suffix_lens[b] keys of its own in row b of page_table; its query
+ * tokens are rows cu_q[b] .. cu_q[b+1] of q (cu_q null: row b, one token each).  The last
+ * query token stands at the last key, the others before it, and each sees the keys up to its own
+ * position (the keys of the query tokens must be in the cache already); a token that sees no
+ * key gives 0.  out = softmax(q k * scale) v, rows as q; rows of no sequence are not written.
+ * n_heads a multiple of the cache's n_kv_heads; head_dim 64 or 128; page_size 16, 32, 64, 128 or
+ * 256; q and out in the cache's type; scale > 0.  Keys that no query token sees may hold any
+ * value (NaN too) where they lie past the prefix or past a sequence's keys; keys that some token
+ * of a sequence sees must have finite values.  workspace: 256-byte aligned, at least
+ * vx_shared_prefix_attention_workspace(a) bytes, used by this call alone until it is done. */
+typedef struct vx_shared_prefix_args {
+  vx_kv_pages cache;
+  const void* q;
+  void* out;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const int32_t *prefix_pages, *page_table, *suffix_lens, *cu_q;
+  int32_t* status;
+  void* workspace;
+  int64_t workspace_bytes, table_stride;
+  int32_t n_tokens, n_seqs, n_heads, prefix_len, max_pages;
+  float scale;
+} vx_shared_prefix_args;
+int64_t vx_shared_prefix_attention_workspace(const vx_shared_prefix_args* a);
+int vx_shared_prefix_attention(const vx_shared_prefix_args* a, void* stream, char* err, size_t err_len);
+
+/* One token from each row of logits.  Per row: w_i = exp((x_i - max) / temperature), 0 for -inf
+ * and NaN; in descending order (equal logits in index order) min_p drops w < min_p (the most
+ * likely token has w = 1), top_k keeps the first k (0 or less: all), top_p the shortest run whose
+ * mass reaches top_p of what is left (1 or more: all; at least one token); the token is the
+ * first whose running mass reaches u * (kept mass), u in [0, 1).  With top_k 0 and min_p 0 this is
+ * the order and rule of sampleTopP (src/engine.ts:247-289), masses in f64.  temperature <= 0: the
+ * first of the largest.  out[r]: the index, -1 for a row without a finite or +inf logit.
+ * Each setting is a device array by row, or (array null) the value beside it for all rows.
+ * n_cols <= 262144. */
+typedef struct vx_sample_args {
+  const void* logits;
+  const double* u; /* [n_rows] */
+  const float *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  int32_t* out;
+  int64_t row_stride;
+  double temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all;
+  int32_t dtype; /* F16, BF16 or F32 */
+  int32_t n_rows, n_cols, reserved[2];
+} vx_sample_args;
+int vx_sample_logits(const vx_sample_args* a, void* stream, char* err, size_t err_len);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,314 @@
+// vx_ops.cu — host side of the serving operators that run on the caller's device memory:
+// argument checks, launch shapes and launches (the kernels: k_rope_append.cuh,
+// k_prefix_attn.cuh, k_sample.cuh).
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/voxtral_b200.h"
+#include "k_prefix_attn.cuh"
+#include "k_rope_append.cuh"
+#include "k_sample.cuh"
+
+namespace {
+
+using namespace vx;
+
+struct Err {
+  char* buf;
+  size_t n;
+  int fail(int code, const char* fmt, ...) const {
+    if (buf && n) {
+      va_list ap;
+      va_start(ap, fmt);
+      vsnprintf(buf, n, fmt, ap);
+      va_end(ap);
+    }
+    return code;
+  }
+  int ok() const {
+    if (buf && n) buf[0] = 0;
+    return VX_OK;
+  }
+};
+
+constexpr int kMaxDevices = 64;
+
+int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  n = known[dev].load();
+  if (!n && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(n);
+  return n;
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int elem_size(int dtype) { return dtype == 2 ? 4 : 2; }
+bool row_strides(int dtype, int64_t a, int64_t b) {
+  const int unit = 16 / elem_size(dtype);
+  return a % unit == 0 && b % unit == 0;
+}
+
+// Shared memory beyond 48 KB needs an attribute, once per kernel and device.
+template <typename K>
+cudaError_t allow_smem(K kernel, std::atomic<int> (&done)[kMaxDevices], size_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+  if (done[dev].load() >= (int)bytes) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done[dev].store((int)bytes);
+  return e;
+}
+
+// Programmatic dependent launch: the kernel may be set up while the one before it drains and
+// waits for its results in griddep_wait.
+template <typename P>
+cudaError_t launch(void (*kernel)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P& p, int cluster = 1) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+int check_cache(const vx_kv_pages& c, const Err& e) {
+  if (!c.k || !c.v) return e.fail(VX_E_INVALID, "cache: k and v must be device pointers");
+  if (c.dtype != 0 && c.dtype != 1) return e.fail(VX_E_INVALID, "cache: dtype %d (0 F16 or 1 BF16)", c.dtype);
+  if (c.n_pages < 1 || c.n_kv_heads < 1 || c.page_size < 1 || c.n_kv_heads > 65535)
+    return e.fail(VX_E_RANGE, "cache: %d pages of %d slots, %d heads", c.n_pages, c.page_size, c.n_kv_heads);
+  if (!aligned(c.k) || !aligned(c.v) || !row_strides(0, c.k_page_stride, c.k_head_stride) || !row_strides(0, c.k_slot_stride, 0) ||
+      !row_strides(0, c.v_page_stride, c.v_head_stride) || !row_strides(0, c.v_slot_stride, 0))
+    return e.fail(VX_E_INVALID, "cache: rows must start on 16-byte boundaries");
+  if (std::min({c.k_page_stride, c.k_head_stride, c.k_slot_stride, c.v_page_stride, c.v_head_stride, c.v_slot_stride}) < 0)
+    return e.fail(VX_E_INVALID, "cache: negative strides");
+  return VX_OK;
+}
+
+int launch_error(const Err& e, cudaError_t ce) {
+  return e.fail(VX_E_CUDA, "launch: %s", cudaGetErrorString(ce));
+}
+
+// ------------------------------------------------------------------ rope + append
+template <typename TI, typename TC>
+cudaError_t launch_append(const append::Params& p, int interleaved, cudaStream_t s) {
+  const dim3 grid(p.n_tokens), block(128);
+  return interleaved ? launch(append::k_rope_append<TI, TC, true>, grid, block, 0, s, p)
+                     : launch(append::k_rope_append<TI, TC, false>, grid, block, 0, s, p);
+}
+
+// ------------------------------------------------------------------ attention
+struct Plan {
+  int nt;         // row tiles of 8 nt rows
+  long long tiles;
+  int splits;
+  int64_t bytes;
+};
+
+int check_attention(const vx_shared_prefix_args& a, const Err& e) {
+  const vx_kv_pages& c = a.cache;
+  int rc = check_cache(c, e);
+  if (rc) return rc;
+  if (c.head_dim != 64 && c.head_dim != 128) return e.fail(VX_E_RANGE, "head_dim %d (64 or 128)", c.head_dim);
+  if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1)))
+    return e.fail(VX_E_RANGE, "page_size %d (16, 32, 64, 128 or 256)", c.page_size);
+  if (a.n_tokens < 0 || a.n_seqs < 0) return e.fail(VX_E_RANGE, "%d tokens of %d sequences", a.n_tokens, a.n_seqs);
+  if (a.n_heads < 1 || a.n_heads % c.n_kv_heads)
+    return e.fail(VX_E_RANGE, "n_heads %d is not a multiple of n_kv_heads %d", a.n_heads, c.n_kv_heads);
+  if (a.prefix_len < 0 || a.prefix_len > (1 << 30) || a.max_pages < 0 || (int64_t)a.max_pages * c.page_size > (1 << 30))
+    return e.fail(VX_E_RANGE, "prefix_len %d, %d pages of %d own keys: at most 2^30 each", a.prefix_len, a.max_pages, c.page_size);
+  if (!(a.scale > 0.f) || a.scale > 1e30f) return e.fail(VX_E_RANGE, "scale %g must be positive", (double)a.scale);
+  if (!a.cu_q && a.n_tokens != a.n_seqs)
+    return e.fail(VX_E_INVALID, "%d tokens for %d sequences: cu_q is needed", a.n_tokens, a.n_seqs);
+  return VX_OK;
+}
+
+// Launch shape of arguments that check_attention has let pass.
+int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
+  const vx_kv_pages& c = a.cache;
+  const int group = a.n_heads / c.n_kv_heads, sms = sm_count();
+  if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
+  pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
+  const int rows = 8 * pl.nt;
+  pl.tiles = a.cu_q ? (long long)a.n_tokens * group / rows + a.n_seqs : (long long)a.n_seqs * ((group + rows - 1) / rows);
+  if (pl.tiles > 0x7fffffff) return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
+  // key ranges: enough CTAs for two waves of two an SM, 256 keys a range at least
+  const long long items = std::max(1ll, pl.tiles * c.n_kv_heads);
+  const long long keys = (long long)a.prefix_len + (long long)a.max_pages * c.page_size;
+  pl.splits = (int)std::max(1ll, std::min({(4ll * sms + items - 1) / items, (keys + 255) / 256, 64ll}));
+  pl.bytes = pl.splits == 1 ? 0 : (int64_t)pl.splits * a.n_tokens * a.n_heads * (c.head_dim + 2) * 4;
+  return VX_OK;
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch_rows(const pattn::Params& p, long long tiles, cudaStream_t s) {
+  static std::atomic<int> done[kMaxDevices];
+  // the rings, and the warps' f32 states that take their place at the end
+  constexpr int bytes = std::max(pattn::row_smem<D>(), pattn::kRowWarps * 8 * NT * D * 4);
+  cudaError_t ce = allow_smem(pattn::k_attn_rows<T, D, NT>, done, bytes);
+  if (ce != cudaSuccess) return ce;
+  return launch(pattn::k_attn_rows<T, D, NT>, dim3((unsigned)tiles, p.n_kv, p.splits), dim3(pattn::kRowWarps * 32), bytes, s, p);
+}
+
+template <typename T, int D>
+cudaError_t launch_attention(pattn::Params p, const Plan& pl, cudaStream_t s) {
+  p.splits = pl.splits;
+  p.direct = pl.splits == 1;
+  cudaError_t ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.tiles, s)
+                   : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.tiles, s) : launch_rows<T, D, 4>(p, pl.tiles, s);
+  if (ce != cudaSuccess || p.direct) return ce;
+  const long long rows = (long long)p.n_tokens * p.n_heads;
+  return launch(pattn::k_attn_join<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, p);
+}
+
+// ------------------------------------------------------------------ sampling
+template <typename T>
+cudaError_t launch_sample(const sample::Params& p, int rows, int cluster, cudaStream_t s) {
+  static std::atomic<int> done[kMaxDevices];
+  const size_t bytes = sizeof(sample::Smem) + (size_t)p.slice * 4;
+  cudaError_t ce = allow_smem(sample::k_sample<T>, done, sizeof(sample::Smem) + sample::kMaxSlice * 4);
+  if (ce != cudaSuccess) return ce;
+  return launch(sample::k_sample<T>, dim3((unsigned)rows * cluster), dim3(sample::kThreads), bytes, s, p, cluster);
+}
+
+}  // namespace
+
+extern "C" int vx_rope_append_kv(const vx_rope_append_args* ap, void* stream, char* err, size_t err_len) {
+  const Err e{err, err_len};
+  if (!ap) return e.fail(VX_E_INVALID, "arguments are null");
+  const vx_rope_append_args& a = *ap;
+  const vx_kv_pages& c = a.cache;
+  int rc = check_cache(c, e);
+  if (rc) return rc;
+  if (a.dtype < 0 || a.dtype > 2) return e.fail(VX_E_INVALID, "dtype %d (0 F16, 1 BF16, 2 F32)", a.dtype);
+  if (c.head_dim < 16 || c.head_dim > 512 || c.head_dim % 16)
+    return e.fail(VX_E_RANGE, "head_dim %d must be a multiple of 16 in [16, 512]", c.head_dim);
+  if (a.rot_dim < 0 || a.rot_dim > c.head_dim || a.rot_dim % 16)
+    return e.fail(VX_E_RANGE, "rot_dim %d must be a multiple of 16 up to head_dim %d", a.rot_dim, c.head_dim);
+  if (a.n_tokens < 0 || a.n_heads < 0 || a.n_seqs < 0 || a.max_pages < 0)
+    return e.fail(VX_E_RANGE, "%d tokens, %d heads, %d sequences of %d pages", a.n_tokens, a.n_heads, a.n_seqs, a.max_pages);
+  if ((int64_t)(a.n_heads + 2LL * c.n_kv_heads) * (c.head_dim / 16) > 0x7fffffff)
+    return e.fail(VX_E_RANGE, "%d heads of %d values are too many", a.n_heads, c.head_dim);
+  if (a.n_tokens == 0) return e.ok();
+  if (!a.k || !a.v || !a.page_table || !a.seq_ids || !a.positions || (a.n_heads && (!a.q || !a.q_out)) || (a.rot_dim && !a.rope_freq))
+    return e.fail(VX_E_INVALID, "q, k, v, q_out, page_table, seq_ids, positions and rope_freq must be device pointers");
+  if (!aligned(a.q) || !aligned(a.k) || !aligned(a.v) || !aligned(a.q_out) || !row_strides(a.dtype, a.q_token_stride, a.q_head_stride) ||
+      !row_strides(a.dtype, a.k_token_stride, a.k_head_stride) || !row_strides(a.dtype, a.v_token_stride, a.v_head_stride) ||
+      !row_strides(0, a.q_out_token_stride, a.q_out_head_stride))
+    return e.fail(VX_E_INVALID, "rows of q, k, v and q_out must start on 16-byte boundaries");
+  append::Params p{};
+  p.q = a.q; p.k = a.k; p.v = a.v; p.q_out = a.q_out; p.k_pages = c.k; p.v_pages = c.v;
+  p.q_tok = a.q_token_stride; p.q_head = a.q_head_stride; p.k_tok = a.k_token_stride; p.k_head = a.k_head_stride;
+  p.v_tok = a.v_token_stride; p.v_head = a.v_head_stride; p.qo_tok = a.q_out_token_stride; p.qo_head = a.q_out_head_stride;
+  p.kp_page = c.k_page_stride; p.kp_head = c.k_head_stride; p.kp_slot = c.k_slot_stride;
+  p.vp_page = c.v_page_stride; p.vp_head = c.v_head_stride; p.vp_slot = c.v_slot_stride;
+  p.page_table = a.page_table; p.seq_ids = a.seq_ids; p.positions = a.positions; p.freq = a.rope_freq; p.status = a.status;
+  p.table_stride = a.table_stride; p.n_tokens = a.n_tokens; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads;
+  p.head_dim = c.head_dim; p.rot_dim = a.rot_dim; p.page_size = c.page_size; p.n_pages = c.n_pages; p.n_seqs = a.n_seqs;
+  p.max_pages = a.max_pages;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t ce;
+  if (c.dtype == 0)
+    ce = a.dtype == 0 ? launch_append<__half, __half>(p, a.interleaved, s)
+         : a.dtype == 1 ? launch_append<__nv_bfloat16, __half>(p, a.interleaved, s) : launch_append<float, __half>(p, a.interleaved, s);
+  else
+    ce = a.dtype == 0 ? launch_append<__half, __nv_bfloat16>(p, a.interleaved, s)
+         : a.dtype == 1 ? launch_append<__nv_bfloat16, __nv_bfloat16>(p, a.interleaved, s)
+                        : launch_append<float, __nv_bfloat16>(p, a.interleaved, s);
+  return ce == cudaSuccess ? e.ok() : launch_error(e, ce);
+}
+
+extern "C" int64_t vx_shared_prefix_attention_workspace(const vx_shared_prefix_args* a) {
+  Plan pl{};
+  const Err e{nullptr, 0};
+  return a && check_attention(*a, e) == VX_OK && plan_attention(*a, pl, e) == VX_OK ? pl.bytes : 0;
+}
+
+extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void* stream, char* err, size_t err_len) {
+  const Err e{err, err_len};
+  if (!ap) return e.fail(VX_E_INVALID, "arguments are null");
+  const vx_shared_prefix_args& a = *ap;
+  const vx_kv_pages& c = a.cache;
+  int rc = check_attention(a, e);
+  if (rc) return rc;
+  if (a.n_tokens == 0 || a.n_seqs == 0) return e.ok();
+  if (!a.q || !a.out || !a.suffix_lens || (a.max_pages && !a.page_table) || (a.prefix_len && !a.prefix_pages))
+    return e.fail(VX_E_INVALID, "q, out, suffix_lens, page_table and prefix_pages must be device pointers");
+  if (!aligned(a.q) || !aligned(a.out) || !row_strides(0, a.q_token_stride, a.q_head_stride) ||
+      !row_strides(0, a.out_token_stride, a.out_head_stride))
+    return e.fail(VX_E_INVALID, "rows of q and out must start on 16-byte boundaries");
+  Plan pl{};
+  rc = plan_attention(a, pl, e);
+  if (rc) return rc;
+  if (pl.bytes && (!a.workspace || (reinterpret_cast<uintptr_t>(a.workspace) & 255) || a.workspace_bytes < pl.bytes))
+    return e.fail(VX_E_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)pl.bytes);
+  pattn::Params p{};
+  p.q = a.q; p.out = a.out;
+  p.q_tok = a.q_token_stride; p.q_head = a.q_head_stride; p.o_tok = a.out_token_stride; p.o_head = a.out_head_stride;
+  p.k = pattn::Pages{c.k, c.k_page_stride, c.k_head_stride, c.k_slot_stride};
+  p.v = pattn::Pages{c.v, c.v_page_stride, c.v_head_stride, c.v_slot_stride};
+  p.prefix_pages = a.prefix_pages; p.page_table = a.page_table; p.suffix_lens = a.suffix_lens; p.cu_q = a.cu_q;
+  p.table_stride = a.table_stride; p.status = a.status;
+  p.part_o = (float*)a.workspace;
+  p.part_ml = (float*)a.workspace + (size_t)pl.splits * a.n_tokens * a.n_heads * c.head_dim;
+  p.n_tokens = a.n_tokens; p.n_seqs = a.n_seqs; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads; p.group = a.n_heads / c.n_kv_heads;
+  p.prefix_len = a.prefix_len; p.page_size = c.page_size; p.n_pages = c.n_pages; p.max_pages = a.max_pages;
+  p.scale_log2 = a.scale * pattn::kLog2e;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t ce;
+  if (c.dtype == 0) ce = c.head_dim == 64 ? launch_attention<__half, 64>(p, pl, s) : launch_attention<__half, 128>(p, pl, s);
+  else ce = c.head_dim == 64 ? launch_attention<__nv_bfloat16, 64>(p, pl, s) : launch_attention<__nv_bfloat16, 128>(p, pl, s);
+  return ce == cudaSuccess ? e.ok() : launch_error(e, ce);
+}
+
+extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* err, size_t err_len) {
+  const Err e{err, err_len};
+  if (!ap) return e.fail(VX_E_INVALID, "arguments are null");
+  const vx_sample_args& a = *ap;
+  constexpr int most = sample::kMaxSlice * sample::kMaxCluster;
+  if (a.dtype < 0 || a.dtype > 2) return e.fail(VX_E_INVALID, "dtype %d (0 F16, 1 BF16, 2 F32)", a.dtype);
+  if (a.n_rows < 0 || a.n_cols < 1 || a.n_cols > most || a.row_stride < 0)
+    return e.fail(VX_E_RANGE, "%d rows of %d logits (1 to %d), stride %lld", a.n_rows, a.n_cols, most, (long long)a.row_stride);
+  if (!a.temperature && !(a.temperature_all >= 0.0 && a.temperature_all <= 3e38))
+    return e.fail(VX_E_RANGE, "temperature %g must be 0 or more", a.temperature_all);
+  if (!a.top_p && !(a.top_p_all >= 0.0)) return e.fail(VX_E_RANGE, "top_p %g must be 0 or more", a.top_p_all);
+  if (!a.min_p && !(a.min_p_all >= 0.0 && a.min_p_all <= 1.0))
+    return e.fail(VX_E_RANGE, "min_p %g must be in [0, 1]", a.min_p_all);
+  if (a.n_rows == 0) return e.ok();
+  if (!a.logits || !a.u || !a.out) return e.fail(VX_E_INVALID, "logits, u and out must be device pointers");
+  if (reinterpret_cast<uintptr_t>(a.logits) % elem_size(a.dtype)) return e.fail(VX_E_INVALID, "logits must be aligned to their type");
+  const int sms = sm_count();
+  if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
+  int cluster = 1;
+  while (cluster < sample::kMaxCluster &&
+         ((a.n_cols + cluster - 1) / cluster > sample::kMaxSlice ||
+          ((long long)a.n_rows * cluster * 2 <= sms && (a.n_cols + cluster - 1) / cluster > 4096)))
+    cluster *= 2;
+  if ((long long)a.n_rows * cluster > 0x7fffffff) return e.fail(VX_E_RANGE, "%d rows are too many for one call", a.n_rows);
+  sample::Params p{};
+  p.logits = a.logits; p.stride = a.row_stride; p.u = a.u;
+  p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.top_k = a.top_k;
+  p.temperature1 = a.temperature_all; p.top_p1 = a.top_p_all; p.min_p1 = a.min_p_all; p.top_k1 = a.top_k_all;
+  p.out = a.out; p.n = a.n_cols;
+  p.slice = (a.n_cols + cluster - 1) / cluster;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t ce = a.dtype == 0 ? launch_sample<__half>(p, a.n_rows, cluster, s)
+                         : a.dtype == 1 ? launch_sample<__nv_bfloat16>(p, a.n_rows, cluster, s) : launch_sample<float>(p, a.n_rows, cluster, s);
+  return ce == cudaSuccess ? e.ok() : launch_error(e, ce);
+}

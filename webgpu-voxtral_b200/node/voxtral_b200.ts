@@ -26,6 +26,31 @@ const vx_config = koffi.struct('vx_config', {
 });
 koffi.opaque('vx_handle');
 
+// Serving operators on the caller's device memory: pointers are device addresses.
+const vx_kv_pages = koffi.struct('vx_kv_pages', {
+  k: 'void *', v: 'void *', k_page_stride: 'int64', k_head_stride: 'int64', k_slot_stride: 'int64',
+  v_page_stride: 'int64', v_head_stride: 'int64', v_slot_stride: 'int64', n_pages: 'int32', n_kv_heads: 'int32',
+  page_size: 'int32', head_dim: 'int32', dtype: 'int32', reserved: 'int32',
+});
+koffi.struct('vx_rope_append_args', {
+  cache: vx_kv_pages, q: 'void *', k: 'void *', v: 'void *', q_out: 'void *', q_token_stride: 'int64', q_head_stride: 'int64',
+  k_token_stride: 'int64', k_head_stride: 'int64', v_token_stride: 'int64', v_head_stride: 'int64',
+  q_out_token_stride: 'int64', q_out_head_stride: 'int64', page_table: 'void *', seq_ids: 'void *', positions: 'void *',
+  rope_freq: 'void *', status: 'void *', table_stride: 'int64', dtype: 'int32', n_tokens: 'int32', n_heads: 'int32',
+  n_seqs: 'int32', max_pages: 'int32', rot_dim: 'int32', interleaved: 'int32', reserved: 'int32',
+});
+koffi.struct('vx_shared_prefix_args', {
+  cache: vx_kv_pages, q: 'void *', out: 'void *', q_token_stride: 'int64', q_head_stride: 'int64',
+  out_token_stride: 'int64', out_head_stride: 'int64', prefix_pages: 'void *', page_table: 'void *', suffix_lens: 'void *',
+  cu_q: 'void *', status: 'void *', workspace: 'void *', workspace_bytes: 'int64', table_stride: 'int64',
+  n_tokens: 'int32', n_seqs: 'int32', n_heads: 'int32', prefix_len: 'int32', max_pages: 'int32', scale: 'float',
+});
+koffi.struct('vx_sample_args', {
+  logits: 'void *', u: 'void *', temperature: 'void *', top_p: 'void *', min_p: 'void *', top_k: 'void *', out: 'void *',
+  row_stride: 'int64', temperature_all: 'double', top_p_all: 'double', min_p_all: 'double', top_k_all: 'int32',
+  dtype: 'int32', n_rows: 'int32', n_cols: 'int32', reserved: koffi.array('int32', 2),
+});
+
 // One entry per declaration of include/voxtral_b200.h.
 export const vx = {
   default_config: lib.func('void vx_default_config(_Out_ vx_config *cfg)'),
@@ -72,6 +97,10 @@ export const vx = {
   selftest_gemm: lib.func('int vx_selftest_gemm(vx_handle *h, int32_t M, int32_t N, int32_t K, int32_t bn, int32_t maxSplits, uint64_t seed, _Out_ double *err)'),
   selftest_top_p: lib.func('int vx_selftest_top_p(vx_handle *h, const float *logits, int32_t n, int32_t lo, int32_t hi, double topP, double temperature, const double *u, int32_t nDraws, _Out_ int32_t *out)'),
   lm_head_argmax_noalloc: lib.func('int vx_lm_head_argmax_noalloc(const uint16_t *w, const float *x, int32_t rows, int32_t dim, int32_t *outIndex, float *outValue, void *stream, _Out_ char *err, size_t errLen)'),
+  rope_append_kv: lib.func('int vx_rope_append_kv(const vx_rope_append_args *a, void *stream, _Out_ char *err, size_t errLen)'),
+  shared_prefix_attention_workspace: lib.func('int64_t vx_shared_prefix_attention_workspace(const vx_shared_prefix_args *a)'),
+  shared_prefix_attention: lib.func('int vx_shared_prefix_attention(const vx_shared_prefix_args *a, void *stream, _Out_ char *err, size_t errLen)'),
+  sample_logits: lib.func('int vx_sample_logits(const vx_sample_args *a, void *stream, _Out_ char *err, size_t errLen)'),
 };
 
 const DIM = 3072;
