@@ -17,7 +17,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libvoxtral_b200.so")
 SOURCES = ["vx_engine.cu", "vx_noalloc.cu", "vx_ops.cu"]
-DEPS = ["vx_engine.cu", "vx_noalloc.cu", "vx_ops.cu", "vx_ops.cuh", "k_rope_append.cuh", "k_prefix_attn.cuh", "k_sample.cuh",
+DEPS = ["vx_engine.cu", "vx_noalloc.cu", "vx_ops.cu", "vx_ops.cuh", "vx_tcgen05.cuh", "k_rope_append.cuh", "k_prefix_attn.cuh", "k_sample.cuh",
         "k_gemv.cuh", "k_attn.cuh", "k_misc.cuh", "k_step.cuh", "k_gemm.cuh", "k_codec.cuh",
         "vx_codec.cuh", "vx_common.cuh", "vx_rng.h"]
 

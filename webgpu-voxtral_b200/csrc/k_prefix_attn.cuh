@@ -15,6 +15,7 @@
 // over the keys), their sum l is not.
 #pragma once
 #include "vx_ops.cuh"
+#include "vx_tcgen05.cuh"
 
 namespace vx {
 namespace pattn {
@@ -323,6 +324,335 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_attn_rows(const __grid_const
       if (M != -INFINITY) *reinterpret_cast<float4*>(p.part_o + row * D + d) = acc;
       if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * row) = make_float2(M, L);
     }
+  }
+}
+
+// ---------------------------------------------------------------- tiles of 128 rows
+// One CTA takes up to 256 query rows of one K/V head (two tiles of 128) against one range of
+// 128-key tiles, on the tensor cores: S = Q K^T and O += P V as tcgen05.mma with f32 accumulators
+// in TMEM, P written back into TMEM over S as the A operand of the second product.
+//   OWN = false: the rows of all sequences against the shared prefix, which is so read and
+//                multiplied once for the whole batch;
+//   OWN = true:  the rows of one sequence against its prefix and own keys, causally.
+// Warps 0-3 and 4-7 each do the softmax of one tile, a thread a row (no shuffles); warp 8 brings
+// the pages in by TMA; one thread of warp 9 issues the products.  While one tile's softmax runs,
+// the other tile's products do.  The reference exponent of a row only moves when its maximum grows
+// by more than 2^8 (weights stay below 2^8, far inside f16's and f32's range), so that O in TMEM is
+// hardly ever rescaled.
+//
+// Bound: for a wide batch the tensor cores and the exponentials (a 128 x 128 tile needs 1024 cycles
+// of products at head_dim 128 and 1024 of ex2), for a narrow one the reading of K and V.
+constexpr int kTile = 128;
+constexpr int kTileThreads = 320;
+template <int D>
+struct TileCfg {
+  static constexpr int kSlot = kTile * D * 2;                       // a K or V tile, or a tile of Q
+  static constexpr int kSlots = D == 128 ? 5 : 8;
+  static constexpr size_t kSmem = (size_t)(2 + kSlots) * kSlot + 1024 + 256;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <typename T, int D, bool OWN>
+__global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_constant__ CUtensorMap kmap,
+                                                                const __grid_constant__ CUtensorMap vmap,
+                                                                const __grid_constant__ Params p) {
+  using E = ops::Elem<T>;
+  using C = TileCfg<D>;
+  constexpr uint32_t kIdescQK = (1u << 4) | (E::kIdescType << 7) | (E::kIdescType << 10) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);
+  constexpr uint32_t kIdescPV = (1u << 4) | (E::kIdescType << 7) | (E::kIdescType << 10) | (1u << 16) | ((D >> 3) << 17) | ((kTile >> 4) << 24);
+  constexpr uint32_t kHalf = kTile * 128;   // bytes of 64 columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  uint8_t* ring = smem + 2 * C::kSlot;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kSlot);
+  uint64_t* empty = full + C::kSlots;
+  uint64_t* q_full = empty + C::kSlots;
+  uint64_t* s_full = q_full + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* tail = o_done + 1;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  volatile int* abort = &s_abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], kTile);
+    }
+    mbar_init(o_done, 1);
+    mbar_init(tail, 1);
+    fence_mbar_init();
+    s_abort = 0;
+    prefetch_tmap(&kmap);
+    prefetch_tmap(&vmap);
+  }
+  griddep_launch();
+  griddep_wait();
+
+  // ---- the rows and keys of this CTA (the same in every thread)
+  int b = 0, ti = blockIdx.x;
+  int tok0 = 0, n_rows, own = 0, first_lim = p.prefix_len, last_lim = p.prefix_len;
+  if (OWN) {
+    if (!find_tile(p, blockIdx.x, 2 * kTile, lane, b, ti)) return;
+    tok0 = p.cu_q[b];
+    const int nq = p.cu_q[b + 1] - tok0;
+    const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
+    own = max(0, min(given, cap));
+    n_rows = min(2 * kTile, nq * p.group - ti * 2 * kTile);
+    if ((given > cap || tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) && threadIdx.x == 0) ops::report(p.status, kDevBadIndex);
+    if (tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) return;
+    first_lim = p.prefix_len + own - nq + 1;
+    last_lim = max(0, first_lim + (ti * 2 * kTile + n_rows - 1) / p.group);
+  } else {
+    n_rows = min((long long)2 * kTile, (long long)p.n_tokens * p.group - (long long)ti * 2 * kTile);
+  }
+  const int row0 = ti * 2 * kTile;                       // first row: token tok0 + row / group, head row % group
+  const int n_pre = (min(p.prefix_len, last_lim) + kTile - 1) / kTile;
+  const int n_all = n_pre + (max(0, last_lim - p.prefix_len) + kTile - 1) / kTile;
+  const int per = (n_all + p.splits - 1) / p.splits;
+  const int t0 = split * per, n = max(0, min(n_all, t0 + per) - t0);
+  const int n_tiles = n_rows > kTile ? 2 : 1;
+
+  if (warp == 9) tc::tmem_alloc(&s_tmem, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 384};
+
+  if (warp == 8) {
+    // ---- pages into the ring: K of tile 0, V of tile 0, K of tile 1, ...
+    const int box = min(p.page_size, kTile);
+    int issued = 0, tails = 0;
+    bool ok = true;
+    for (int it = 0; ok && it < 2 * n; ++it) {
+      const int s = it % C::kSlots, t = t0 + (it >> 1);
+      const bool is_v = it & 1;
+      if (it >= C::kSlots) {
+        int go = lane == 0 ? ops::wait_phase(&empty[s], (uint32_t)(it / C::kSlots - 1) & 1u, abort, p.status, kDevTimeoutEmpty) : 0;
+        ok = __shfl_sync(0xffffffffu, go, 0);
+        if (!ok) break;
+      }
+      const bool pre = t < n_pre;
+      const int key = kTile * (pre ? t : t - n_pre), valid = min(kTile, (pre ? p.prefix_len : own) - key);
+      const int boxes = (valid + box - 1) / box;
+      // a tile that ends early: V's missing rows are zeroed (0 x NaN), K's scores are masked
+      const bool zero = is_v && valid < kTile;
+      uint64_t* bar = zero ? tail : &full[s];
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * D * 2));
+      __syncwarp();
+      const uint32_t dst = smem_u32(ring + s * C::kSlot);
+      if (lane < boxes) {
+        const int at = key + lane * box, lp = at / p.page_size;
+        int page = -1;
+        if (pre) page = p.prefix_pages[lp];
+        else if (lp < p.max_pages) page = p.page_table[(long long)b * p.table_stride + lp];
+        if (page < 0 || page >= p.n_pages) {
+          ops::report(p.status, kDevBadIndex);
+          page = p.n_pages;   // past the map's end: reads as zero
+        }
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_4d(dst + h * kHalf + lane * box * 128, is_v ? &vmap : &kmap, h * 64, at % p.page_size, kvh, page, bar);
+      }
+      issued = it + 1;
+      if (zero) {
+        __syncwarp();
+        ops::wait_landed(tail, tails & 1, p.status);
+        ++tails;
+        for (int x = lane; x < (kTile - valid) * 8 * (D / 64); x += 32) {
+          const int h = x / ((kTile - valid) * 8), c = x % ((kTile - valid) * 8);
+          *reinterpret_cast<uint4*>(ring + s * C::kSlot + h * kHalf + valid * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+      }
+      __syncwarp();
+    }
+    // after a failure nobody may be waiting for the last copies: they land before the CTA ends
+    if (!ok || *abort)
+      for (int it = max(0, issued - C::kSlots); it < issued; ++it) ops::wait_landed(&full[it % C::kSlots], (uint32_t)(it / C::kSlots) & 1u, p.status);
+  } else if (warp == 9) {
+    if (lane == 0 && n > 0) {
+      const uint32_t q_s = smem_u32(smem), r_s = smem_u32(ring);
+      const auto qk = [&](int i, int slot) {
+        const uint32_t q = q_s + i * C::kSlot, k = r_s + slot * C::kSlot;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+          tc::tc_mma(t_s[i], tc::sw128_desc(q + off), tc::sw128_desc(k + off), kIdescQK, kk != 0);
+        }
+        tc::tc_commit(&s_full[i]);
+      };
+      bool ok = ops::wait_phase(q_full, 0, abort, p.status, kDevTimeoutFull) && ops::wait_phase(&full[0], 0, abort, p.status, kDevTimeoutFull);
+      if (ok) {
+        tc::tc_fence_after();
+        for (int i = 0; i < n_tiles; ++i) qk(i, 0);
+        tc::tc_commit(&empty[0]);
+      }
+      for (int j = 0; ok && j < n; ++j) {
+        const int iv = 2 * j + 1, ik = iv + 1, sv = iv % C::kSlots, sk = ik % C::kSlots;
+        for (int i = 0; ok && i < n_tiles; ++i) {
+          ok = ops::wait_phase(&p_full[i], (uint32_t)j & 1u, abort, p.status, kDevTimeoutRed) &&
+               (i || ops::wait_phase(&full[sv], (uint32_t)(iv / C::kSlots) & 1u, abort, p.status, kDevTimeoutFull));
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t v = r_s + sv * C::kSlot;
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            tc::tc_mma_ta(t_o[i], t_s[i] + kk * 8, tc::sw128_mn_desc(v + kk * 2048, kHalf), kIdescPV, (j | kk) != 0);
+          if (i == n_tiles - 1) tc::tc_commit(&empty[sv]);
+          if (j + 1 < n) {
+            if (i == 0) {
+              ok = ops::wait_phase(&full[sk], (uint32_t)(ik / C::kSlots) & 1u, abort, p.status, kDevTimeoutFull);
+              if (!ok) break;
+              tc::tc_fence_after();
+            }
+            qk(i, sk);
+            if (i == n_tiles - 1) tc::tc_commit(&empty[sk]);
+          }
+        }
+      }
+      tc::tc_commit(o_done);
+      if (!ok) ops::wait_landed(o_done, 0, p.status);   // products already issued end before TMEM is freed
+    }
+  } else {
+    // ---- Q into shared memory (128-byte swizzle), then the softmax of one tile
+    const int wg = warp >> 2, row = threadIdx.x & (kTile - 1);
+    for (int x = row; x < kTile * (D / 8); x += kTile) {
+      const int r = x / (D / 8), c = x % (D / 8), lr = wg * kTile + r;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (lr < n_rows) {
+        const int g = (row0 + lr) % p.group;
+        const long long tok = tok0 + (row0 + lr) / p.group;
+        v = *reinterpret_cast<const uint4*>((const T*)p.q + tok * p.q_tok + (long long)(kvh * p.group + g) * p.q_head + c * 8);
+      }
+      *reinterpret_cast<uint4*>(smem + wg * C::kSlot + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_async_smem();
+    mbar_arrive(q_full);
+
+    if (wg < n_tiles) {
+      const int lr = wg * kTile + row;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const int lim = OWN ? first_lim + (row0 + min(lr, n_rows - 1)) / p.group : p.prefix_len;   // keys that the row sees
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        ok = ops::wait_phase(&s_full[wg], (uint32_t)j & 1u, abort, p.status, kDevTimeoutAcc);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        float s[kTile];
+        tc::tmem_ld128(t_s[wg] + lanes, s);
+        const int t = t0 + j;
+        const bool pre = t < n_pre;
+        const int key = kTile * (pre ? t : t - n_pre);
+        const int see = min((pre ? p.prefix_len : own), lim - (pre ? 0 : p.prefix_len)) - key;   // keys of this tile that count
+        if (__any_sync(0xffffffffu, see < kTile)) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i)
+            if (i >= see) s[i] = -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+          const float m_new = fmaxf(m, top), f = ex2(m == m_new ? 0.f : m - m_new);
+          l *= f;
+          m = m_new;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            uint32_t u[32];
+            tc::tmem_ld32(t_o[wg] + lanes + c, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * f);
+            tc::tmem_st32(t_o[wg] + lanes + c, u);
+          }
+        }
+        const float m_use = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kTile; c += 64) {
+          uint32_t u[32];
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) {
+            const float x = ex2(fmaf(s[c + i], p.scale_log2, -m_use)), y = ex2(fmaf(s[c + i + 1], p.scale_log2, -m_use));
+            sum[i & 2] += x;
+            sum[(i & 2) + 1] += y;
+            u[i >> 1] = E::pack(x, y);
+          }
+          tc::tmem_st32(t_s[wg] + lanes + c / 2, u);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_st_wait();
+        tc::tc_fence_before();
+        mbar_arrive(&p_full[wg]);
+      }
+      if (ok && n > 0) ok = __all_sync(0xffffffffu, ops::wait_phase(o_done, 0, abort, p.status, kDevTimeoutAcc));
+      if (ok) {
+        tc::tc_fence_after();
+        const bool live = lr < n_rows;
+        const int g = (row0 + min(lr, n_rows - 1)) % p.group;
+        const long long tok = tok0 + (row0 + min(lr, n_rows - 1)) / p.group;
+        const int head = kvh * p.group + g;
+        const long long at = (long long)(p.split0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        if (live && !p.direct) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          if (n > 0) {
+            tc::tmem_ld32(t_o[wg] + lanes + c, o);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (live && p.direct) {
+            uint4* dst = reinterpret_cast<uint4*>((T*)p.out + tok * p.o_tok + (long long)head * p.o_head + c);
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              dst[i / 8] = make_uint4(E::pack(o[i] * inv, o[i + 1] * inv), E::pack(o[i + 2] * inv, o[i + 3] * inv),
+                                      E::pack(o[i + 4] * inv, o[i + 5] * inv), E::pack(o[i + 6] * inv, o[i + 7] * inv));
+          } else if (live && m != -INFINITY) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 512);
   }
 }
 

@@ -67,8 +67,8 @@ cudaError_t allow_smem(K kernel, std::atomic<int> (&done)[kMaxDevices], size_t b
 
 // Programmatic dependent launch: the kernel may be set up while the one before it drains and
 // waits for its results in griddep_wait.
-template <typename P>
-cudaError_t launch(void (*kernel)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const P& p, int cluster = 1) {
+template <typename... P, typename... A>
+cudaError_t launch_cluster(int cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -85,7 +85,11 @@ cudaError_t launch(void (*kernel)(P), dim3 grid, dim3 block, size_t smem, cudaSt
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A&... args) {
+  return launch_cluster(1, kernel, grid, block, smem, stream, args...);
 }
 
 int check_cache(const vx_kv_pages& c, const Err& e) {
@@ -115,11 +119,29 @@ cudaError_t launch_append(const append::Params& p, int interleaved, cudaStream_t
 
 // ------------------------------------------------------------------ attention
 struct Plan {
-  int nt;         // row tiles of 8 nt rows
-  long long tiles;
-  int splits;
+  int nt;               // row kernel: tiles of 8 nt rows; 0: not launched
+  long long row_tiles;
+  int row_splits;
+  int own;              // tile kernel over prefix and own keys (1) or the shared prefix alone (0)
+  long long pairs;      // tile kernel: pairs of 128-row tiles; 0: not launched
+  int tile_splits;
   int64_t bytes;
 };
+
+// Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's
+// share of the key tiles least, a range's start and end counted as two tiles.
+int tile_splits(long long items, long long tiles, int sms) {
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 2.0);
+    if (cost < least * 0.999) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
 
 int check_attention(const vx_shared_prefix_args& a, const Err& e) {
   const vx_kv_pages& c = a.cache;
@@ -144,16 +166,61 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   const vx_kv_pages& c = a.cache;
   const int group = a.n_heads / c.n_kv_heads, sms = sm_count();
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
-  pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
-  const int rows = 8 * pl.nt;
-  pl.tiles = a.cu_q ? (long long)a.n_tokens * group / rows + a.n_seqs : (long long)a.n_seqs * ((group + rows - 1) / rows);
-  if (pl.tiles > 0x7fffffff) return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
-  // key ranges: enough CTAs for two waves of two an SM, 256 keys a range at least
-  const long long items = std::max(1ll, pl.tiles * c.n_kv_heads);
-  const long long keys = (long long)a.prefix_len + (long long)a.max_pages * c.page_size;
-  pl.splits = (int)std::max(1ll, std::min({(4ll * sms + items - 1) / items, (keys + 255) / 256, 64ll}));
-  pl.bytes = pl.splits == 1 ? 0 : (int64_t)pl.splits * a.n_tokens * a.n_heads * (c.head_dim + 2) * 4;
+  const long long own_keys = (long long)a.max_pages * c.page_size, rows = (long long)a.n_tokens * group;
+  pl = Plan{};
+  // The tile kernel multiplies 128 rows at once; below 64 rows a sequence the row kernel's tiles
+  // of 32 waste less.  One token a sequence: the prefix goes to the tile kernel, all sequences together.
+  pl.own = a.cu_q && rows >= 64ll * a.n_seqs;
+  if (pl.own) {
+    pl.pairs = rows / 256 + a.n_seqs;
+    pl.tile_splits = tile_splits(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128 + (own_keys + 127) / 128, sms);
+  } else {
+    if (!a.cu_q && a.n_seqs > 1 && a.prefix_len >= 128) {
+      pl.pairs = (rows + 255) / 256;
+      pl.tile_splits = tile_splits(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
+    }
+    const long long keys = own_keys + (pl.pairs ? 0 : a.prefix_len);
+    if (keys || !pl.pairs) {
+      pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
+      const int tile = 8 * pl.nt;
+      pl.row_tiles = a.cu_q ? rows / tile + a.n_seqs : (long long)a.n_seqs * ((group + tile - 1) / tile);
+      // enough CTAs for two waves of two an SM, 256 keys a range at least
+      const long long items = std::max(1ll, pl.row_tiles * c.n_kv_heads);
+      pl.row_splits = (int)std::max(1ll, std::min({(4ll * sms + items - 1) / items, (keys + 255) / 256, 64ll}));
+    }
+  }
+  if (std::max(pl.pairs, pl.row_tiles) > 0x7fffffff)
+    return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
+  const int splits = pl.tile_splits + pl.row_splits;
+  pl.bytes = splits == 1 ? 0 : (int64_t)splits * a.n_tokens * a.n_heads * (c.head_dim + 2) * 4;
   return VX_OK;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Map of a page pool: boxes of 64 values x up to 128 slots of one head of one page.
+cudaError_t encode_pages(CUtensorMap* map, const vx_kv_pages& c, const pattn::Pages& g) {
+  static std::atomic<void*> known{nullptr};
+  void* fn = known.load();
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t ce = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (ce != cudaSuccess) return ce;
+    if (!fn || q != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    known.store(fn);
+  }
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)g.slot * 2, (cuuint64_t)g.head * 2, (cuuint64_t)g.page * 2};
+  for (int i = 0; i < 3; ++i)
+    if (dims[i + 1] == 1) strides[i] = 16;   // never stepped over; the caller's may be anything
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(c.page_size, 128), 1, 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = ((EncodeTiledFn)fn)(map, c.dtype ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                                         const_cast<void*>(g.base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 template <typename T, int D, int NT>
@@ -165,14 +232,36 @@ cudaError_t launch_rows(const pattn::Params& p, long long tiles, cudaStream_t s)
   if (ce != cudaSuccess) return ce;
   return launch(pattn::k_attn_rows<T, D, NT>, dim3((unsigned)tiles, p.n_kv, p.splits), dim3(pattn::kRowWarps * 32), bytes, s, p);
 }
+template <typename T, int D, bool OWN>
+cudaError_t launch_tiles(const pattn::Params& p, const vx_kv_pages& c, long long pairs, cudaStream_t s) {
+  static std::atomic<int> done[kMaxDevices];
+  constexpr size_t bytes = pattn::TileCfg<D>::kSmem;
+  cudaError_t ce = allow_smem(pattn::k_attn_tiles<T, D, OWN>, done, bytes);
+  CUtensorMap km, vm;
+  if (ce == cudaSuccess) ce = encode_pages(&km, c, p.k);
+  if (ce == cudaSuccess) ce = encode_pages(&vm, c, p.v);
+  if (ce != cudaSuccess) return ce;
+  return launch(pattn::k_attn_tiles<T, D, OWN>, dim3((unsigned)pairs, p.n_kv, p.splits), dim3(pattn::kTileThreads), bytes, s, km, vm, p);
+}
 
 template <typename T, int D>
-cudaError_t launch_attention(pattn::Params p, const Plan& pl, cudaStream_t s) {
-  p.splits = pl.splits;
-  p.direct = pl.splits == 1;
-  cudaError_t ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.tiles, s)
-                   : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.tiles, s) : launch_rows<T, D, 4>(p, pl.tiles, s);
+cudaError_t launch_attention(pattn::Params p, const vx_kv_pages& c, const Plan& pl, cudaStream_t s) {
+  const int all = pl.tile_splits + pl.row_splits;
+  p.direct = all == 1;
+  cudaError_t ce = cudaSuccess;
+  if (pl.pairs) {
+    p.splits = pl.tile_splits;
+    ce = pl.own ? launch_tiles<T, D, true>(p, c, pl.pairs, s) : launch_tiles<T, D, false>(p, c, pl.pairs, s);
+    p.split0 = pl.tile_splits;
+    p.own_only = 1;
+  }
+  if (ce == cudaSuccess && pl.row_tiles) {
+    p.splits = pl.row_splits;
+    ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.row_tiles, s)
+         : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.row_tiles, s) : launch_rows<T, D, 4>(p, pl.row_tiles, s);
+  }
   if (ce != cudaSuccess || p.direct) return ce;
+  p.splits = all;
   const long long rows = (long long)p.n_tokens * p.n_heads;
   return launch(pattn::k_attn_join<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, p);
 }
@@ -184,7 +273,7 @@ cudaError_t launch_sample(const sample::Params& p, int rows, int cluster, cudaSt
   const size_t bytes = sizeof(sample::Smem) + (size_t)p.slice * 4;
   cudaError_t ce = allow_smem(sample::k_sample<T>, done, sizeof(sample::Smem) + sample::kMaxSlice * 4);
   if (ce != cudaSuccess) return ce;
-  return launch(sample::k_sample<T>, dim3((unsigned)rows * cluster), dim3(sample::kThreads), bytes, s, p, cluster);
+  return launch_cluster(cluster, sample::k_sample<T>, dim3((unsigned)rows * cluster), dim3(sample::kThreads), bytes, s, p);
 }
 
 }  // namespace
@@ -266,14 +355,14 @@ extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void*
   p.prefix_pages = a.prefix_pages; p.page_table = a.page_table; p.suffix_lens = a.suffix_lens; p.cu_q = a.cu_q;
   p.table_stride = a.table_stride; p.status = a.status;
   p.part_o = (float*)a.workspace;
-  p.part_ml = (float*)a.workspace + (size_t)pl.splits * a.n_tokens * a.n_heads * c.head_dim;
+  p.part_ml = (float*)a.workspace + (size_t)(pl.tile_splits + pl.row_splits) * a.n_tokens * a.n_heads * c.head_dim;
   p.n_tokens = a.n_tokens; p.n_seqs = a.n_seqs; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads; p.group = a.n_heads / c.n_kv_heads;
   p.prefix_len = a.prefix_len; p.page_size = c.page_size; p.n_pages = c.n_pages; p.max_pages = a.max_pages;
   p.scale_log2 = a.scale * pattn::kLog2e;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t ce;
-  if (c.dtype == 0) ce = c.head_dim == 64 ? launch_attention<__half, 64>(p, pl, s) : launch_attention<__half, 128>(p, pl, s);
-  else ce = c.head_dim == 64 ? launch_attention<__nv_bfloat16, 64>(p, pl, s) : launch_attention<__nv_bfloat16, 128>(p, pl, s);
+  if (c.dtype == 0) ce = c.head_dim == 64 ? launch_attention<__half, 64>(p, c, pl, s) : launch_attention<__half, 128>(p, c, pl, s);
+  else ce = c.head_dim == 64 ? launch_attention<__nv_bfloat16, 64>(p, c, pl, s) : launch_attention<__nv_bfloat16, 128>(p, c, pl, s);
   return ce == cudaSuccess ? e.ok() : launch_error(e, ce);
 }
 
