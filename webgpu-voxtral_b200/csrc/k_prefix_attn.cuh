@@ -62,6 +62,30 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+typedef unsigned long long f32x2;   // two f32 in a register pair: one instruction for both
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -357,6 +381,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+// One row from shared to global memory; returns when the shared memory has been read.
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, int bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename T, int D, bool OWN>
@@ -533,24 +563,39 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       tc::tc_commit(o_done);
       if (!ok) ops::wait_landed(o_done, 0, p.status);   // products already issued end before TMEM is freed
     }
-  } else {
+  } else if (warp < 8) {
     // ---- Q into shared memory (128-byte swizzle), then the softmax of one tile
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1);
-    for (int x = row; x < kTile * (D / 8); x += kTile) {
-      const int r = x / (D / 8), c = x % (D / 8), lr = wg * kTile + r;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (lr < n_rows) {
-        const int g = (row0 + lr) % p.group;
-        const long long tok = tok0 + (row0 + lr) / p.group;
-        v = *reinterpret_cast<const uint4*>((const T*)p.q + tok * p.q_tok + (long long)(kvh * p.group + g) * p.q_head + c * 8);
+    {
+      constexpr int CH = D / 8, STEP = kTile / CH;   // 16-byte chunks of a row; this thread's rows are STEP apart
+      const int c = row % CH;
+      int g = (row0 + wg * kTile + row / CH) % p.group;
+      long long tok = tok0 + (row0 + wg * kTile + row / CH) / p.group;
+      const int step_g = STEP % p.group, step_tok = STEP / p.group;
+      const T* src = (const T*)p.q + (long long)kvh * p.group * p.q_head + c * 8;
+      uint4 v[CH];
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const bool in = wg * kTile + row / CH + k * STEP < n_rows;
+        v[k] = in ? *reinterpret_cast<const uint4*>(src + tok * p.q_tok + g * p.q_head) : make_uint4(0, 0, 0, 0);
+        g += step_g;
+        tok += step_tok;
+        if (g >= p.group) {
+          g -= p.group;
+          ++tok;
+        }
       }
-      *reinterpret_cast<uint4*>(smem + wg * C::kSlot + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int r = row / CH + k * STEP;
+        *reinterpret_cast<uint4*>(smem + wg * C::kSlot + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+      }
     }
     fence_async_smem();
     mbar_arrive(q_full);
 
     if (wg < n_tiles) {
-      const int lr = wg * kTile + row;
+      const int lr = wg * kTile + row;   // this thread's row
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int lim = OWN ? first_lim + (row0 + min(lr, n_rows - 1)) / p.group : p.prefix_len;   // keys that the row sees
       float m = -INFINITY, l = 0.f;
@@ -575,7 +620,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < kTile; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+        for (int i = 4; i + 8 <= kTile; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        mx[0] = max3(mx[0], s[kTile - 4], s[kTile - 3]);
+        mx[1] = max3(mx[1], s[kTile - 2], s[kTile - 1]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         if (j == 0) {
           m = top;
@@ -584,30 +633,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
           l *= f;
           m = m_new;
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            uint32_t u[32];
-            tc::tmem_ld32(t_o[wg] + lanes + c, o);
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            uint32_t u[16];
+            tc::tmem_ld16(t_o[wg] + lanes + c, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = __float_as_uint(o[i] * f);
-            tc::tmem_st32(t_o[wg] + lanes + c, u);
+            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f);
+            tc::tmem_st16(t_o[wg] + lanes + c, u);
           }
         }
         const float m_use = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2), off2 = pack2(-m_use, -m_use);
+        f32x2 sum[2] = {pack2(l, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < kTile; c += 64) {
           uint32_t u[32];
 #pragma unroll
           for (int i = 0; i < 64; i += 2) {
-            const float x = ex2(fmaf(s[c + i], p.scale_log2, -m_use)), y = ex2(fmaf(s[c + i + 1], p.scale_log2, -m_use));
-            sum[i & 2] += x;
-            sum[(i & 2) + 1] += y;
+            float x, y;
+            unpack2(fma2(pack2(s[c + i], s[c + i + 1]), scale2, off2), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(x, y));
             u[i >> 1] = E::pack(x, y);
           }
           tc::tmem_st32(t_s[wg] + lanes + c / 2, u);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        {
+          float x, y;
+          unpack2(add2(sum[0], sum[1]), x, y);
+          l = x + y;
+        }
         tc::tmem_st_wait();
         tc::tc_fence_before();
         mbar_arrive(&p_full[wg]);
@@ -616,12 +672,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       if (ok) {
         tc::tc_fence_after();
         const bool live = lr < n_rows;
-        const int g = (row0 + min(lr, n_rows - 1)) % p.group;
-        const long long tok = tok0 + (row0 + min(lr, n_rows - 1)) / p.group;
-        const int head = kvh * p.group + g;
+        const long long tok = tok0 + (row0 + lr) / p.group;
+        const int head = kvh * p.group + (row0 + lr) % p.group;
         const long long at = (long long)(p.split0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
         if (live && !p.direct) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
+        // rows to memory by one bulk copy each, staged in the ring (free now); 16 bytes of padding
+        // keep the threads' rows on different banks
+        const int row_bytes = p.direct ? D * 2 : D * 4;
+        uint8_t* stage = ring + (size_t)lr * (row_bytes + 16);
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
@@ -631,18 +690,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
-          if (live && p.direct) {
-            uint4* dst = reinterpret_cast<uint4*>((T*)p.out + tok * p.o_tok + (long long)head * p.o_head + c);
+          if (p.direct) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
-              dst[i / 8] = make_uint4(E::pack(o[i] * inv, o[i + 1] * inv), E::pack(o[i + 2] * inv, o[i + 3] * inv),
-                                      E::pack(o[i + 4] * inv, o[i + 5] * inv), E::pack(o[i + 6] * inv, o[i + 7] * inv));
-          } else if (live && m != -INFINITY) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + at * D + c);
+              *reinterpret_cast<uint4*>(stage + (c + i) * 2) =
+                  make_uint4(E::pack(o[i] * inv, o[i + 1] * inv), E::pack(o[i + 2] * inv, o[i + 3] * inv),
+                             E::pack(o[i + 4] * inv, o[i + 5] * inv), E::pack(o[i + 6] * inv, o[i + 7] * inv));
+          } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) dst[i / 4] = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(stage + (c + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
-          __syncwarp();
+        }
+        fence_async_smem();
+        if (live && (p.direct || m != -INFINITY)) {
+          void* dst = p.direct ? (void*)((T*)p.out + tok * p.o_tok + (long long)head * p.o_head) : (void*)(p.part_o + at * D);
+          bulk_s2g(dst, smem_u32(stage), row_bytes);
         }
       }
     }

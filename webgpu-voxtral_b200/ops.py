@@ -18,95 +18,108 @@ transpose(1, 2).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
+import threading
 
 import torch
 
 from .engine import VX_OK, VoxtralError, load_library
 
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_INT = torch.int32
 _CACHE = "2P6q6i"                                # vx_kv_pages
 _APPEND = struct.Struct("@" + _CACHE + "4P8q5Pq8i")   # vx_rope_append_args
 _PREFIX = struct.Struct("@" + _CACHE + "2P4q6P2q5if")  # vx_shared_prefix_args
 _SAMPLE = struct.Struct("@7Pq3d6i")              # vx_sample_args
 _ERR = 256
+_local = threading.local()
 
 
 def _refuse(message: str):
     raise VoxtralError(-1, message)
 
 
+@functools.lru_cache(maxsize=None)
 def _library():
     L = load_library()
-    if not hasattr(L, "_ops_bound"):
-        for name in ("vx_rope_append_kv", "vx_shared_prefix_attention", "vx_sample_logits"):
-            fn = getattr(L, name)
-            fn.restype = ctypes.c_int
-            fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]
-        L.vx_shared_prefix_attention_workspace.restype = ctypes.c_int64
-        L.vx_shared_prefix_attention_workspace.argtypes = [ctypes.c_char_p]
-        L._ops_bound = True
+    for name in ("vx_rope_append_kv", "vx_shared_prefix_attention", "vx_sample_logits"):
+        fn = getattr(L, name)
+        fn.restype = ctypes.c_int
+        fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]
+    L.vx_shared_prefix_attention_workspace.restype = ctypes.c_int64
+    L.vx_shared_prefix_attention_workspace.argtypes = [ctypes.c_char_p]
     return L
 
 
-def _call(fn, args: bytes, device):
-    err = ctypes.create_string_buffer(_ERR)
-    rc = fn(args, torch.cuda.current_stream(device).cuda_stream, err, _ERR)
+def _call(fn, args: bytes, device: int):
+    """fn on torch's current stream of the device, which is made current for the call."""
+    try:
+        err = _local.err
+    except AttributeError:
+        err = _local.err = ctypes.create_string_buffer(_ERR)
+    if device == torch.cuda.current_device():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device), err, _ERR)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(device), err, _ERR)
     if rc != VX_OK:
         raise VoxtralError(rc, err.value.decode())
 
 
-def _on(device):
-    """The device made current for the call where it is not."""
-    return torch.cuda.device(device)
-
-
-def _same_place(device, **tensors):
-    if device.type != "cuda":
-        _refuse(f"tensors must be on a CUDA device, not {device}")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _refuse(f"{name} is on {t.device}, other arguments on {device}")
+def _same_place(names: str, *tensors):
+    """The device that holds them all."""
+    device = tensors[0].get_device()
+    for i, t in enumerate(tensors):
+        if t is not None and (t.get_device() != device or device < 0):
+            first, name = names.split()[0], names.split()[i]
+            _refuse(f"{name} must be on a CUDA device, not {t.device}" if device < 0 else f"{name} is on {t.device}, {first} on cuda:{device}")
+    return device
 
 
 def _rows(name, t, dims, *dtypes):
-    if t.dim() != dims:
-        _refuse(f"{name} must have {dims} dimensions, not {t.dim()}")
+    """Shape and strides of a tensor of rows."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != dims:
+        _refuse(f"{name} must have {dims} dimensions, not {len(shape)}")
     if t.dtype not in dtypes:
         _refuse(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    if stride[-1] != 1 and shape[-1] > 1:
         _refuse(f"{name}: the last dimension must be contiguous")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{name} requires a gradient, which this operator does not compute")
+    return shape, stride
 
 
-def _ints(name, t, n=None):
-    if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
-        _refuse(f"{name} must be a contiguous int32 tensor of one dimension")
-    if n is not None and t.shape[0] != n:
-        _refuse(f"{name} must have {n} elements, not {t.shape[0]}")
+def _vector(name, t, dtype, n=None):
+    shape = t.shape
+    if len(shape) != 1 or t.dtype is not dtype or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous {dtype} tensor of one dimension, not {t.dtype} {tuple(shape)}")
+    if n is not None and shape[0] != n:
+        _refuse(f"{name} must have {n} elements, not {shape[0]}")
 
 
 def _cache(k_pages, v_pages):
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        _rows(name, t, 4, torch.float16, torch.bfloat16)
-    if k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
-        _refuse("k_pages and v_pages must have one shape and type")
-    n, kv, page, d = k_pages.shape
-    ks, vs = k_pages.stride(), v_pages.stride()
-    return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], n, kv, page, d, _DTYPE[k_pages.dtype], 0)
+    shape, ks = _rows("k_pages", k_pages, 4, torch.float16, torch.bfloat16)
+    shape_v, vs = _rows("v_pages", v_pages, 4, k_pages.dtype)
+    if shape != shape_v:
+        _refuse(f"k_pages {tuple(shape)} and v_pages {tuple(shape_v)} must have one shape")
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], *shape, _DTYPE[k_pages.dtype], 0)
 
 
 def _table(page_table):
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    """Rows, columns and row stride of a page table."""
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype is not _INT or (shape[1] > 1 and stride[1] != 1):
         _refuse("page_table must be an int32 tensor [n_seqs, pages] with contiguous rows")
+    return shape[0], shape[1], stride[0]
 
 
 def _status(status):
     if status is None:
         return 0
-    if status.dtype != torch.int32 or status.numel() != 1:
+    if status.dtype is not _INT or status.numel() != 1:
         _refuse("status must be an int32 tensor of one element")
     return status.data_ptr()
 
@@ -120,44 +133,36 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     padding, of which nothing is written).  rope_freq: f32 [rot_dim / 2], the angle of pair i at
     position p is p * rope_freq[i]; pairs are neighbours (interleaved) or the two halves.
     Returns the rotated q in the cache's type (q_out, if given; it may be q itself)."""
-    _rows("k", k, 3, *_DTYPE)
-    _rows("v", v, 3, k.dtype)
+    shape, ks = _rows("k", k, 3, *_DTYPE)
+    shape_v, vs = _rows("v", v, 3, k.dtype)
     cache = _cache(k_pages, v_pages)
-    n, kv, d = k.shape
-    if v.shape != k.shape or kv != cache[9] or d != cache[11]:
-        _refuse(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit a cache of {cache[9]} heads of {cache[11]}")
-    _table(page_table)
-    _ints("seq_ids", seq_ids, n)
-    _ints("positions", positions, n)
-    if rope_freq.dtype != torch.float32 or rope_freq.dim() != 1 or not rope_freq.is_contiguous():
-        _refuse("rope_freq must be a contiguous f32 tensor of one dimension")
-    heads, qs, os = 0, (0, 0), (0, 0)
+    n, kv, d = shape
+    if shape_v != shape or kv != cache[9] or d != cache[11]:
+        _refuse(f"k {tuple(shape)} and v {tuple(shape_v)} do not fit a cache of {cache[9]} heads of {cache[11]}")
+    seqs, pages, table_stride = _table(page_table)
+    _vector("seq_ids", seq_ids, _INT, n)
+    _vector("positions", positions, _INT, n)
+    _vector("rope_freq", rope_freq, torch.float32)
+    heads = q_ptr = out_ptr = 0
+    qs = os = (0, 0)
     if q is not None:
-        _rows("q", q, 3, k.dtype)
-        if q.shape[0] != n or q.shape[2] != d:
-            _refuse(f"q {tuple(q.shape)} does not fit k {tuple(k.shape)}")
+        shape_q, qs = _rows("q", q, 3, k.dtype)
+        if shape_q[0] != n or shape_q[2] != d:
+            _refuse(f"q {tuple(shape_q)} does not fit k {tuple(shape)}")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=k_pages.dtype, device=q.device)
-        _rows("q_out", q_out, 3, k_pages.dtype)
-        if q_out.shape != q.shape:
-            _refuse(f"q_out {tuple(q_out.shape)} must have q's shape {tuple(q.shape)}")
-        heads, qs, os = q.shape[1], q.stride(), q_out.stride()
+            q_out = k_pages.new_empty(shape_q)
+        shape_o, os = _rows("q_out", q_out, 3, k_pages.dtype)
+        if shape_o != shape_q:
+            _refuse(f"q_out {tuple(shape_o)} must have q's shape {tuple(shape_q)}")
+        heads, q_ptr, out_ptr = shape_q[1], q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _refuse("q_out without q")
-    device = k.device
-    _same_place(device, q=q, v=v, k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_ids=seq_ids, positions=positions,
-                rope_freq=rope_freq, q_out=q_out, status=status)
-    ks, vs = k.stride(), v.stride()
-    args = _APPEND.pack(*cache, q.data_ptr() if heads else 0, k.data_ptr(), v.data_ptr(), q_out.data_ptr() if heads else 0,
-                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], page_table.data_ptr(), seq_ids.data_ptr(),
-                        positions.data_ptr(), rope_freq.data_ptr(), _status(status), page_table.stride(0), _DTYPE[k.dtype], n, heads,
-                        page_table.shape[0], page_table.shape[1], 2 * rope_freq.shape[0], int(bool(interleaved)), 0)
-    fn = _library().vx_rope_append_kv
-    if device.index == torch.cuda.current_device():
-        _call(fn, args, device)
-    else:
-        with _on(device):
-            _call(fn, args, device)
+    device = _same_place("k q v k_pages v_pages page_table seq_ids positions rope_freq q_out status", k, q, v, k_pages, v_pages,
+                         page_table, seq_ids, positions, rope_freq, q_out, status)
+    _call(_library().vx_rope_append_kv,
+          _APPEND.pack(*cache, q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
+                       page_table.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), rope_freq.data_ptr(), _status(status), table_stride,
+                       _DTYPE[k.dtype], n, heads, seqs, pages, 2 * rope_freq.shape[0], 1 if interleaved else 0, 0), device)
     return q_out
 
 
@@ -172,66 +177,62 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     scale defaults to 1 / sqrt(head_dim).  Returns out, shaped as q; rows past cu_q's last are not
     written, a row that sees no key is 0.  workspace: a uint8 tensor of at least
     shared_prefix_attention_workspace bytes that no other call uses at the same time."""
-    args, device, out = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, scale, out, status)
-    if device.index == torch.cuda.current_device():
-        _prefix_call(args, device, workspace)
-    else:
-        with _on(device):
-            _prefix_call(args, device, workspace)
+    if out is None:
+        out = q.new_empty(q.shape)
+    cache, sizes, pointers, device = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status)
+    need = _workspace_bytes(sizes, device)
+    held = ptr = 0
+    if workspace is not None:
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or workspace.get_device() != device:
+            _refuse(f"workspace must be a contiguous uint8 tensor on cuda:{device}")
+        ptr, held = workspace.data_ptr(), workspace.numel()
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ptr, held = workspace.data_ptr(), need
+    _call(_library().vx_shared_prefix_attention,
+          _PREFIX.pack(*cache, *pointers[:11], ptr, held, pointers[11], *sizes[6:], 1.0 / math.sqrt(sizes[3]) if scale is None else scale),
+          device)
     return out
 
 
 def shared_prefix_attention_workspace(q, k_pages, v_pages, prefix_pages, prefix_len: int, page_table, suffix_lens, *, cu_q=None) -> int:
     """Bytes of workspace that shared_prefix_attention needs for these arguments.  They depend on
     shapes, prefix_len and whether cu_q is given, not on the values."""
-    args, device, _ = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, None, q, None)
-    with _on(device):
-        return _library().vx_shared_prefix_attention_workspace(_PREFIX.pack(*args))
+    _, sizes, _, device = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, q, None)
+    return _workspace_bytes(sizes, device)
 
 
-def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, scale, out, status):
+def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status):
+    """(cache, sizes, pointers and strides from q to status and then the table's stride, device)"""
     cache = _cache(k_pages, v_pages)
-    _rows("q", q, 3, k_pages.dtype)
-    if q.shape[2] != cache[11]:
-        _refuse(f"q {tuple(q.shape)} does not fit a cache with head_dim {cache[11]}")
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _rows("out", out, 3, q.dtype)
-    if out.shape != q.shape:
-        _refuse(f"out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-    _table(page_table)
-    seqs = page_table.shape[0]
-    _ints("suffix_lens", suffix_lens, seqs)
-    _ints("prefix_pages", prefix_pages)
+    shape, qs = _rows("q", q, 3, k_pages.dtype)
+    if shape[2] != cache[11]:
+        _refuse(f"q {tuple(shape)} does not fit a cache with head_dim {cache[11]}")
+    shape_o, os = _rows("out", out, 3, k_pages.dtype)
+    if shape_o != shape:
+        _refuse(f"out {tuple(shape_o)} must have q's shape {tuple(shape)}")
+    seqs, pages, table_stride = _table(page_table)
+    _vector("suffix_lens", suffix_lens, _INT, seqs)
+    _vector("prefix_pages", prefix_pages, _INT)
     if prefix_len < 0 or prefix_pages.shape[0] * cache[10] < prefix_len:
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_pages.shape[0]} pages of {cache[10]}")
     if cu_q is not None:
-        _ints("cu_q", cu_q, seqs + 1)
-    device = q.device
-    _same_place(device, k_pages=k_pages, v_pages=v_pages, prefix_pages=prefix_pages, page_table=page_table, suffix_lens=suffix_lens,
-                cu_q=cu_q, out=out, status=status)
-    qs, os = q.stride(), out.stride()
-    args = [*cache, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], prefix_pages.data_ptr(), page_table.data_ptr(),
-            suffix_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), _status(status), 0, 0, page_table.stride(0), q.shape[0], seqs,
-            q.shape[1], prefix_len, page_table.shape[1], 1.0 / math.sqrt(q.shape[2]) if scale is None else scale]
-    return args, device, out
+        _vector("cu_q", cu_q, _INT, seqs + 1)
+    device = _same_place("q k_pages v_pages prefix_pages page_table suffix_lens cu_q out status", q, k_pages, v_pages, prefix_pages,
+                         page_table, suffix_lens, cu_q, out, status)
+    sizes = (*cache[8:13], cu_q is not None, shape[0], seqs, shape[1], prefix_len, pages)
+    pointers = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], prefix_pages.data_ptr(), page_table.data_ptr(),
+                suffix_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), _status(status), table_stride)
+    return cache, sizes, pointers, device
 
 
-_WORKSPACE = 25   # place of the workspace pointer in vx_shared_prefix_args; its size comes next
-
-
-def _prefix_call(args, device, workspace):
-    L = _library()
-    if workspace is None:
-        need = L.vx_shared_prefix_attention_workspace(_PREFIX.pack(*args))
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
-        _refuse(f"workspace must be a contiguous uint8 tensor on {device}")
-    if workspace is not None:
-        args[_WORKSPACE] = workspace.data_ptr()
-        args[_WORKSPACE + 1] = workspace.numel()
-    _call(L.vx_shared_prefix_attention, _PREFIX.pack(*args), device)
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(sizes, device):
+    """The library's answer for these sizes (n_pages, kv heads, page, head_dim, dtype, ragged, tokens, sequences,
+    heads, prefix, pages); only sizes enter it."""
+    args = _PREFIX.pack(256, 256, *[sizes[3]] * 6, *sizes[:5], 0, *[0] * 9, 256 if sizes[5] else 0, *[0] * 4, *sizes[6:], 1.0)
+    with torch.cuda.device(device):
+        return _library().vx_shared_prefix_attention_workspace(args)
 
 
 def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
@@ -243,34 +244,31 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     running mass reaches u times the kept mass.  temperature 0 takes the first.  Each setting is a
     number, or a tensor by row (f32; top_k int32).  Returns int32 [n_rows]; -1 for a row whose
     logits are all -inf or NaN."""
-    _rows("logits", logits, 2, *_DTYPE)
-    rows = logits.shape[0]
-    if u.dim() != 1 or u.dtype != torch.float64 or not u.is_contiguous() or u.shape[0] != rows:
-        _refuse(f"u must be a contiguous float64 tensor of {rows} elements")
-    device = logits.device
-    each, one = [], []
+    shape, stride = _rows("logits", logits, 2, *_DTYPE)
+    rows, cols = shape
+    if u.dtype is not torch.float64 or u.shape != (rows,) or not u.is_contiguous():
+        _refuse(f"u must be a contiguous float64 tensor of {rows} elements, not {u.dtype} {tuple(u.shape)}")
+    tensors, each, one = [logits, u], [], []
     for name, v, kind in (("temperature", temperature, torch.float32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
-                          ("top_k", top_k, torch.int32)):
+                          ("top_k", top_k, _INT)):
         if isinstance(v, torch.Tensor):
-            if v.dtype != kind or v.dim() != 1 or not v.is_contiguous() or v.shape[0] != rows or v.device != device:
-                _refuse(f"{name} must be a number or a contiguous {kind} tensor of {rows} elements on {device}")
+            if v.dtype is not kind or v.shape != (rows,) or not v.is_contiguous():
+                _refuse(f"{name} must be a number or a contiguous {kind} tensor of {rows} elements, not {v.dtype} {tuple(v.shape)}")
+            tensors.append(v)
             each.append(v.data_ptr())
             one.append(0)
         else:
             each.append(0)
             one.append(v)
-    if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=device)
-    _ints("out", out, rows)
-    _same_place(device, u=u, out=out)
     if not -2**31 <= one[3] < 2**31:
         _refuse(f"top_k {one[3]} does not fit 32 bits")
-    args = _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), logits.stride(0), one[0], one[1], one[2], int(one[3]),
-                        _DTYPE[logits.dtype], rows, logits.shape[1], 0, 0)
-    fn = _library().vx_sample_logits
-    if device.index == torch.cuda.current_device():
-        _call(fn, args, device)
+    if out is None:
+        out = torch.empty(rows, dtype=_INT, device=logits.device)
     else:
-        with _on(device):
-            _call(fn, args, device)
+        _vector("out", out, _INT, rows)
+        tensors.append(out)
+    device = _same_place("logits u setting setting setting setting out", *tensors)
+    _call(_library().vx_sample_logits,
+          _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), stride[0], one[0], one[1], one[2], int(one[3]),
+                       _DTYPE[logits.dtype], rows, cols, 0, 0), device)
     return out
