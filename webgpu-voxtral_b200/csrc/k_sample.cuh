@@ -15,12 +15,14 @@
 // hundred.
 //
 // No sort of the row.  The row lies in the shared memory of a cluster of 1 to 8 CTAs.  One pass
-// puts each survivor's count and mass into one of 1024 bins, linear in log w; sums over the bins
-// find the bin in which a count or mass is reached.  Where the whole head up to that bin is at
-// most 2048 tokens it is gathered and sorted exactly, and all three limits are found in the
-// sorted list.  Otherwise only the tokens of the bin in question are; a bin with more than 2048
-// is binned again by the bits of the logits, down to a run of equal logits, where the order is
-// the index order.
+// puts each survivor's count and mass into one of 2048 bins, linear in log w; running sums over
+// the bins (each CTA sums a share of them over the cluster) find the bin in which a count or mass
+// is reached.  Where the whole head up to that bin is at most 512 tokens it is gathered into one
+// CTA, sorted exactly, and all three limits are found in the sorted list; with top-k that head is
+// found from counts alone, so only its tokens need an exponential.  Otherwise the tokens of the
+// bin in question are gathered, binned again by their order key (logit, then index) and the few of
+// one such bin sorted.  A bin of more than 1024 tokens is first binned again over the cluster by the
+// same key; runs of equal logits need nothing of their own, as their keys differ in the index.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -32,9 +34,12 @@ namespace sample {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
-constexpr int kBins = kThreads;        // one a thread
-constexpr int kList = 2 * kThreads;    // tokens sorted at once, two a thread
+constexpr int kThreads = 512;
+constexpr int kBins = 2048;
+constexpr int kSub = kThreads;         // second-level bins, one a thread
+constexpr int kHead = kThreads;        // tokens sorted at once, one a thread
+constexpr int kList = 1024;            // tokens gathered at once
+constexpr int kFew = 96;               // tokens of a list that are sorted rather than binned again
 constexpr int kMaxSlice = 32768;       // logits a CTA holds
 constexpr int kMaxCluster = 8;
 constexpr float kRangeLog2 = 45.f;     // w below 2^-45 rounds to mass 0
@@ -51,389 +56,669 @@ struct Params {
   int n, slice;
 };
 
+// Where a running count or mass reaches a target.
+struct Hit {
+  uint32_t bin, cnt_before, cnt;
+  u64 mass_before;
+};
+template <int N>
+struct Bins {
+  uint32_t cnt[N], lo[N], hi[N];       // counts, and masses in two words
+};
 struct Smem {
-  uint32_t cnt[kBins], lo[kBins], hi[kBins];   // this CTA's bins: count, mass in two words
-  u64 mass_to[kBins];                          // whole row: mass and count up to and with the bin
-  uint32_t cnt_to[kBins];
-  u64 list[kList];
-  u64 scan64[32];
-  uint32_t scan32[32];
-  float red[32];
-  float cta_max;
-  uint32_t key_min, key_max;
-  uint32_t n_list, eq_count;
-  // where a target was reached (one thread writes, all read)
-  int hit_bin;
-  uint32_t hit_cnt_before, hit_cnt;
-  u64 hit_mass_before;
-  int res_idx;
+  Bins<kBins> bins;                    // this CTA's part of the row; then running sums of its share of bins
+  Bins<kSub> sub;
+  u64 list[kList], list2[kList];
+  double exp2_tab[64];                 // 2^(j / 64)
+  u64 scan64[16];
+  uint32_t scan32[16];
+  float red[16];
+  float max_of[kMaxCluster];           // each CTA's, and the totals of each one's share of bins
+  uint32_t tot_cnt[kMaxCluster];
+  u64 tot_mass[kMaxCluster];
+  u64 key_min, key_max;
+  uint32_t n_list, n_list2, n_own, at;
+  Hit hit, list_hit;
+  uint32_t share_cnt;                  // what lies before this CTA's share of bins
+  u64 share_mass;
   u64 res_mass;
-  float x[1];                                  // the CTA's slice of the row
+  int res_idx;
+  alignas(16) float x[4];              // the CTA's slice of the row
 };
 
-__device__ __forceinline__ uint32_t desc_key(float x) {   // ascending in the descending order of x
+// Descending order of the logits, then the index: ascending keys.
+__device__ __forceinline__ uint32_t desc_bits(float x) {
   const uint32_t b = __float_as_uint(x);
   return (b & 0x80000000u) ? b : ~b & 0x7fffffffu;
 }
-__device__ __forceinline__ float from_desc_key(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? k : ~k & 0x7fffffffu);
+__device__ __forceinline__ u64 order_key(float x, int i) { return ((u64)desc_bits(x) << 32) | (uint32_t)i; }
+__device__ __forceinline__ float key_logit(u64 k) {
+  const uint32_t b = (uint32_t)(k >> 32);
+  return __uint_as_float((b & 0x80000000u) ? b : ~b & 0x7fffffffu);
 }
 
-template <typename T>
-__device__ __forceinline__ T block_incl_scan(T v, T* sh) {
+// Running sums of counts and masses over the threads, this thread's included.
+__device__ __forceinline__ void block_scan(Smem& s, uint32_t& c, u64& m) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  if (lane == 31) sh[w] = v;
-  __syncthreads();
-  if (w == 0) {
-    T s = sh[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const T y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
+    const uint32_t y = __shfl_up_sync(0xffffffffu, c, o);
+    const u64 z = __shfl_up_sync(0xffffffffu, m, o);
+    if (lane >= o) {
+      c += y;
+      m += z;
     }
-    sh[lane] = s;
+  }
+  if (lane == 31) {
+    s.scan32[w] = c;
+    s.scan64[w] = m;
   }
   __syncthreads();
-  if (w) v += sh[w - 1];
+  // the warps' totals, 16 of them, summed by every warp for itself
+  uint32_t cw = lane < kThreads / 32 ? s.scan32[lane] : 0u;
+  u64 mw = lane < kThreads / 32 ? s.scan64[lane] : 0ull;
+#pragma unroll
+  for (int o = 1; o < kThreads / 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, cw, o);
+    const u64 z = __shfl_up_sync(0xffffffffu, mw, o);
+    if (lane >= o) {
+      cw += y;
+      mw += z;
+    }
+  }
+  cw = __shfl_sync(0xffffffffu, cw, (w + 31) & 31);
+  mw = __shfl_sync(0xffffffffu, mw, (w + 31) & 31);
+  if (w) {
+    c += cw;
+    m += mw;
+  }
   __syncthreads();
-  return v;
+}
+__device__ __forceinline__ u64 block_scan(Smem& s, u64 m) {
+  uint32_t c = 0;
+  block_scan(s, c, m);
+  return m;
+}
+
+// The cluster of C CTAs that holds a row; one CTA needs no more than its own barrier.
+template <int C>
+__device__ __forceinline__ void cluster_barrier() {
+  if constexpr (C == 1) __syncthreads();
+  else cg::this_cluster().sync();
+}
+template <int C>
+__device__ __forceinline__ Smem* of_rank(Smem& s, int q) {
+  if constexpr (C == 1) return &s;
+  else return cg::this_cluster().map_shared_rank(&s, q);
+}
+template <int C>
+__device__ __forceinline__ int my_rank() {
+  if constexpr (C == 1) return 0;
+  else return (int)cg::this_cluster().block_rank();
 }
 
 struct Row {
-  float mx, bin_scale, cut_log2;   // bin = -(x - mx) * bin_scale; nothing below cut_log2 survives
-  double inv_t, min_p;
-  float c;                         // log2(e) / T
+  float mx, c, bin_scale, cut_log2;    // log2 w = -(mx - x) c; nothing below -cut_log2 survives
+  int sure;                            // every logit of the bins below this one survives
+  double mxd, c64, min_p44;            // 64 log2(e) / T; min_p 2^44
 };
-__device__ __forceinline__ u64 mass_of(const Row& r, float x) {
-  const double w = x == r.mx ? 1.0 : exp(((double)x - (double)r.mx) * r.inv_t);
-  return w >= r.min_p ? (u64)__double2ull_rn(w * 17592186044416.0) : 0ull;
+// 2^(j / 64), rounded.
+__device__ const double kExp2[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
+// round(w 2^44) of a logit within 2^-60 of the largest.  2^(t / 64) by the table and the Taylor sum
+// of the rest, |r| <= 1/2 of a 64th (table-driven exponential, Tang 1989): the fifth power's term is
+// below 4e-14.
+__device__ __forceinline__ double weight44(const Smem& s, const Row& r, float x) {
+  constexpr double a = 0.010830424696249145;   // ln 2 / 64
+  const double t = ((double)x - r.mxd) * r.c64;
+  const double shifted = t + 6755399441055744.0;   // 1.5 * 2^52: the nearest whole number in the low bits
+  const int n = __double2loint(shifted);
+  const double f = t - (shifted - 6755399441055744.0);
+  const double poly = fma(f, fma(f, fma(f, fma(f, a * a * a * a / 24.0, a * a * a / 6.0), a * a / 2.0), a), 1.0);
+  const double v = s.exp2_tab[n & 63] * poly;
+  // times 2^(n / 64 + 44) in the exponent field
+  return __hiloint2double(__double2hiint(v) + (((n >> 6) + 44) << 20), __double2loint(v));
 }
+__device__ __forceinline__ u64 whole(double w44) {   // + 2^52: whole in the mantissa
+  return (u64)__double_as_longlong(w44 + 4503599627370496.0) & 0xfffffffffffffull;
+}
+// Mass of a logit of bin b >= 0, 0 where min-p drops it.
+__device__ __forceinline__ u64 mass_of(const Smem& s, const Row& r, float x, int b) {
+  const double w = weight44(s, r, x);
+  return b < r.sure || w >= r.min_p44 ? whole(w) : 0ull;
+}
+// Mass of a token that is known to survive.
+__device__ __forceinline__ u64 mass_of(const Smem& s, const Row& r, float x) { return whole(weight44(s, r, x)); }
 // Bin of a logit, -1 for one that cannot survive (the exact test is mass_of's).
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
-  if (x == r.mx) return 0;
   const float t = (r.mx - x) * r.c;
-  if (!(t <= r.cut_log2)) return -1;
-  return min(kBins - 1, (int)(t * r.bin_scale));
+  return t <= r.cut_log2 ? min(kBins - 1, (int)(t * r.bin_scale)) : -1;
+}
+// Whether a logit of bin b survives.
+__device__ __forceinline__ bool survives(const Smem& s, const Row& r, float x, int b) {
+  return b < r.sure || mass_of(s, r, x, b) > 0;
 }
 
-__device__ __forceinline__ void bins_clear(Smem& s) {
-  s.cnt[threadIdx.x] = s.lo[threadIdx.x] = s.hi[threadIdx.x] = 0;
+template <int N>
+__device__ __forceinline__ void bins_clear(Bins<N>& b) {
+  for (int i = threadIdx.x; i < N; i += kThreads) b.cnt[i] = b.lo[i] = b.hi[i] = 0;
 }
-__device__ __forceinline__ void bins_add(Smem& s, int b, u64 m) {
-  atomicAdd(&s.cnt[b], 1u);
-  const uint32_t l = (uint32_t)m, old = atomicAdd(&s.lo[b], l);
+template <int N>
+__device__ __forceinline__ void bins_add(Bins<N>& b, int i, u64 m) {
+  atomicAdd(&b.cnt[i], 1u);
+  const uint32_t l = (uint32_t)m, old = atomicAdd(&b.lo[i], l);
   const uint32_t h = (uint32_t)(m >> 32) + (old + l < old ? 1u : 0u);
-  if (h) atomicAdd(&s.hi[b], h);
-}
-// This thread's bin over the whole cluster, then its running sums.
-__device__ __forceinline__ void bins_sum(Smem& s, cg::cluster_group& cl, uint32_t& cnt, u64& mass, uint32_t& cnt_to, u64& mass_to) {
-  cl.sync();
-  cnt = 0;
-  mass = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-    const Smem* o = cl.map_shared_rank(&s, r);
-    cnt += o->cnt[threadIdx.x];
-    mass += ((u64)o->hi[threadIdx.x] << 32) + o->lo[threadIdx.x];
-  }
-  cl.sync();   // every CTA has read the others' bins
-  cnt_to = block_incl_scan<uint32_t>(cnt, s.scan32);
-  mass_to = block_incl_scan<u64>(mass, s.scan64);
+  if (h) atomicAdd(&b.hi[i], h);
 }
 
-// Sorts the first n of the list (ascending, kList at most) in this CTA.
-__device__ void sort_list(Smem& s, int n) {
-  int n2 = 2;
-  while (n2 < n) n2 <<= 1;
-  for (int i = threadIdx.x; i < n2; i += kThreads)
-    if (i >= n) s.list[i] = ~0ull;
-  __syncthreads();
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      const int t = threadIdx.x;
-      if (t < n2 / 2) {
-        const int a = ((t & ~(j - 1)) << 1) | (t & (j - 1)), b = a | j;
-        const u64 x = s.list[a], y = s.list[b];
-        if ((x > y) == ((a & k) == 0)) {
-          s.list[a] = y;
-          s.list[b] = x;
-        }
-      }
-      __syncthreads();
+// Running sums of the row's bins: this CTA's share of them, [rank kBins / C, ...), replaces its bins.
+// Gives the row's total count and mass.
+template <int C>
+__device__ void sum_bins(Smem& s, uint32_t& cnt_all, u64& mass_all) {
+  constexpr int share = kBins / C, per = (share + kThreads - 1) / kThreads;   // bins a thread
+  const int t = threadIdx.x, rank = my_rank<C>();
+  const bool on = t * per < share;
+  cluster_barrier<C>();
+  uint32_t c[per];
+  u64 m[per];
+#pragma unroll
+  for (int j = 0; j < per; ++j) {
+    uint32_t cq[C], lq[C], hq[C];
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      const Smem* o = of_rank<C>(s, q);
+      const int b = rank * share + (on ? t * per + j : 0);
+      cq[q] = o->bins.cnt[b];
+      lq[q] = o->bins.lo[b];
+      hq[q] = o->bins.hi[b];
     }
+    c[j] = 0;
+    m[j] = 0;
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      c[j] += on ? cq[q] : 0u;
+      m[j] += on ? ((u64)hq[q] << 32) + lq[q] : 0ull;
+    }
+  }
+  uint32_t c_to = 0;
+  u64 m_to = 0;
+#pragma unroll
+  for (int j = 0; j < per; ++j) {
+    c_to += c[j];
+    m_to += m[j];
+  }
+  uint32_t c_before = c_to;
+  u64 m_before = m_to;
+  block_scan(s, c_to, m_to);
+  if (t == kThreads - 1)
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      Smem* o = of_rank<C>(s, q);
+      o->tot_cnt[rank] = c_to;
+      o->tot_mass[rank] = m_to;
+    }
+  cluster_barrier<C>();                        // the totals are there, and every CTA has read the others' bins
+  c_before = c_to - c_before;
+  m_before = m_to - m_before;
+  cnt_all = 0;
+  mass_all = 0;
+  uint32_t c_share = 0;
+  u64 m_share = 0;
+#pragma unroll
+  for (int q = 0; q < C; ++q) {
+    if (q < rank) {
+      c_share += s.tot_cnt[q];
+      m_share += s.tot_mass[q];
+    }
+    cnt_all += s.tot_cnt[q];
+    mass_all += s.tot_mass[q];
+  }
+  if (t == 0) {
+    s.share_cnt = c_share;
+    s.share_mass = m_share;
+  }
+  c_before += c_share;
+  m_before += m_share;
+  if (on)
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+      c_before += c[j];
+      m_before += m[j];
+      s.bins.cnt[t * per + j] = c_before;
+      s.bins.lo[t * per + j] = (uint32_t)m_before;
+      s.bins.hi[t * per + j] = (uint32_t)(m_before >> 32);
+    }
+  __syncthreads();
+}
+// The bin in which the target is reached, in s.hit of every CTA.
+template <int C>
+__device__ void find_bin(Smem& s, bool by_count, u64 target) {
+  constexpr int share = kBins / C;
+#pragma unroll
+  for (int b = threadIdx.x; b < share; b += kThreads) {
+    const uint32_t c1 = s.bins.cnt[b], c0 = b ? s.bins.cnt[b - 1] : s.share_cnt;
+    const u64 m1 = ((u64)s.bins.hi[b] << 32) + s.bins.lo[b];
+    const u64 m0 = b ? ((u64)s.bins.hi[b - 1] << 32) + s.bins.lo[b - 1] : s.share_mass;
+    const u64 from = by_count ? (u64)c0 : m0, to = by_count ? (u64)c1 : m1;
+    if (from < target && to >= target)
+#pragma unroll
+      for (int q = 0; q < C; ++q) of_rank<C>(s, q)->hit = Hit{(uint32_t)(my_rank<C>() * share + b), c0, c1 - c0, m0};
+  }
+  cluster_barrier<C>();
 }
 
-// Puts the cluster's tokens for which `take` holds into the list of CTA 0.
+// Calls f(x, i) for every logit of the slice, four at a time (the slice ends in -inf).
 template <typename F>
-__device__ void gather(Smem& s, cg::cluster_group& cl, int base, int n, F take) {
-  Smem* head = cl.map_shared_rank(&s, 0);
-  if (cl.block_rank() == 0 && threadIdx.x == 0) s.n_list = 0;
-  cl.sync();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float x = s.x[i];
-    if (take(x)) head->list[atomicAdd(&head->n_list, 1u) & (kList - 1)] = ((u64)desc_key(x) << 32) | (uint32_t)(base + i);
+__device__ __forceinline__ void each_logit(const Smem& s, int n, F f) {
+#pragma unroll 2
+  for (int v = threadIdx.x; v * 4 < n; v += kThreads) {
+    const float4 x = *reinterpret_cast<const float4*>(&s.x[4 * v]);
+    f(x.x, 4 * v);
+    f(x.y, 4 * v + 1);
+    f(x.z, 4 * v + 2);
+    f(x.w, 4 * v + 3);
   }
-  cl.sync();
 }
 
-// First token in order whose running count (by_count) or mass reaches the target; the row's
-// bins hold it.  Gives its index and the running mass up to and with it, in every CTA.
-__device__ void select(Smem& s, cg::cluster_group& cl, const Row& r, int base, int n, bool by_count, u64 target) {
-  const int t = threadIdx.x;
-  {
-    const u64 to = by_count ? (u64)s.cnt_to[t] : s.mass_to[t];
-    const u64 from = t ? (by_count ? (u64)s.cnt_to[t - 1] : s.mass_to[t - 1]) : 0ull;
-    if (from < target && to >= target) {
-      s.hit_bin = t;
-      s.hit_cnt_before = t ? s.cnt_to[t - 1] : 0u;
-      s.hit_cnt = s.cnt_to[t] - s.hit_cnt_before;
-      s.hit_mass_before = t ? s.mass_to[t - 1] : 0ull;
-    }
+// Puts the cluster's tokens for which `take(x, i)` holds into the list of CTA 0, whose n_list is 0:
+// first into a list of the CTA's own, then those together.
+template <int C, typename F>
+__device__ __forceinline__ void gather(Smem& s, int base, int n, F take) {
+  if constexpr (C > 1) {
+    if (threadIdx.x == 0) s.n_own = 0;
+    __syncthreads();
   }
+  uint32_t* count = C > 1 ? &s.n_own : &s.n_list;
+  u64* list = C > 1 ? s.list2 : s.list;
+  each_logit(s, n, [&](float x, int i) {
+    if (take(x, base + i)) {
+      const uint32_t at = atomicAdd(count, 1u);
+      if (at < (uint32_t)kList) list[at] = order_key(x, base + i);
+    }
+  });
+  if constexpr (C > 1) {
+    __syncthreads();
+    const uint32_t own = min(s.n_own, (uint32_t)kList);
+    Smem* head = of_rank<C>(s, 0);
+    if (threadIdx.x == 0) s.at = own ? atomicAdd(&head->n_list, own) : 0u;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < own; i += kThreads)
+      if (s.at + i < (uint32_t)kList) head->list[s.at + i] = s.list2[i];
+  }
+  cluster_barrier<C>();
+}
+
+// Sorts `c` (at most one a thread) distinct keys: each counts the smaller ones.  Gives this thread's
+// key of the sorted order (~0 past the end).
+__device__ u64 sorted(Smem& s, const u64* list, int c) {
+  const int t = threadIdx.x;
+  // several threads share a key's comparisons where there are few keys
+  int ways = 1;
+  while (ways < 16 && c * ways * 2 <= kThreads) ways *= 2;
+  const int e = t / ways, part = t % ways;
+  const u64 mine = e < c ? list[e] : ~0ull;
+  uint32_t less = 0;
+  for (int i = part; i < c; i += ways) less += list[i] < mine;
+  for (int o = ways >> 1; o > 0; o >>= 1) less += __shfl_xor_sync(0xffffffffu, less, o);
+  __syncthreads();                             // all have read the list before it may be the target
+  if (part == 0 && e < c) s.list2[less] = mine;
   __syncthreads();
-  const int bin = s.hit_bin;
-  uint32_t k0 = 0, k1 = 0xffffffffu;   // desc_key range of the tokens in question, inside the bin
-  const auto member = [&](float x) {
-    const uint32_t k = desc_key(x);
-    return bin_of(r, x) == bin && k >= k0 && k <= k1 && mass_of(r, x) > 0;
-  };
-  // every level takes 10 bits off the span, so the fourth leaves single logits
-  for (int level = 0; level < 8; ++level) {
-    const uint32_t cnt = s.hit_cnt, cnt_before = s.hit_cnt_before;
-    const u64 mass_before = s.hit_mass_before;
-    __syncthreads();
-    if (cnt <= (uint32_t)kList) {
-      gather(s, cl, base, n, member);
-      if (cl.block_rank() == 0) {
-        const int c = (int)cnt;
-        sort_list(s, c);
-        u64 m0 = 0, m1 = 0;
-        if (2 * t < c) m0 = mass_of(r, from_desc_key((uint32_t)(s.list[2 * t] >> 32)));
-        if (2 * t + 1 < c) m1 = mass_of(r, from_desc_key((uint32_t)(s.list[2 * t + 1] >> 32)));
-        const u64 to1 = mass_before + block_incl_scan<u64>(m0 + m1, s.scan64), to0 = to1 - m1;
-        const u64 c0 = by_count ? cnt_before + 2ull * t : to0 - m0, c1 = by_count ? c0 + 1 : to0, c2 = by_count ? c0 + 2 : to1;
-        const bool in0 = 2 * t < c && c0 < target && c1 >= target, in1 = 2 * t + 1 < c && c1 < target && c2 >= target;
-        if (in0 || in1)
-          for (unsigned q = 0; q < cl.num_blocks(); ++q) {
-            Smem* o = cl.map_shared_rank(&s, q);
-            o->res_idx = (int)(uint32_t)s.list[2 * t + (in0 ? 0 : 1)];
-            o->res_mass = in0 ? to0 : to1;
-          }
-      }
-      cl.sync();
-      return;
-    }
-    // too many: the span of their logits, then bins over it
+  const u64 k = t < c ? s.list2[t] : ~0ull;
+  __syncthreads();
+  return k;
+}
+
+// In CTA 0, whose list holds the c <= kList tokens of hit: the first whose running count or mass
+// reaches the target.  Index and running mass to res_idx / res_mass of every CTA.
+template <int C>
+__device__ void resolve_list(Smem& s, const Row& r, int c, uint32_t cnt_before, u64 mass_before, bool by_count, u64 target) {
+  const int t = threadIdx.x;
+  for (int level = 0; level < 8 && c > kFew; ++level) {
+    // bins over the span of the keys; the tokens of the bin in question replace the list.  A bin
+    // holds less than a 256th of the span, so eight rounds end at single keys
     if (t == 0) {
-      s.key_min = 0xffffffffu;
+      s.key_min = ~0ull;
       s.key_max = 0;
+      s.n_list2 = 0;
     }
-    bins_clear(s);
+    bins_clear(s.sub);
     __syncthreads();
-    uint32_t lo = 0xffffffffu, hi = 0;
-    for (int i = t; i < n; i += kThreads)
-      if (member(s.x[i])) {
-        const uint32_t k = desc_key(s.x[i]);
-        lo = min(lo, k);
-        hi = max(hi, k);
+    u64 key[kList / kThreads], lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      const int i = t + j * kThreads;
+      key[j] = i < c ? s.list[i] : ~0ull;
+      if (i < c) {
+        lo = min(lo, key[j]);
+        hi = max(hi, key[j]);
       }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
     if ((t & 31) == 0) {
       atomicMin(&s.key_min, lo);
       atomicMax(&s.key_max, hi);
     }
-    cl.sync();
-    for (unsigned q = 0; q < cl.num_blocks(); ++q) {
-      const Smem* o = cl.map_shared_rank(&s, q);
+    __syncthreads();
+    lo = s.key_min;
+    const int shift = max(0, 64 - __clzll((long long)(s.key_max - lo)) - 9);
+    u64 mass[kList / kThreads];
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j)
+      if (t + j * kThreads < c) {
+        mass[j] = mass_of(s, r, key_logit(key[j]));
+        bins_add(s.sub, (int)((key[j] - lo) >> shift), mass[j]);
+      }
+    __syncthreads();
+    const uint32_t bc = s.sub.cnt[t];
+    const u64 bm = ((u64)s.sub.hi[t] << 32) + s.sub.lo[t];
+    uint32_t c_to = bc;
+    u64 m_to = bm;
+    block_scan(s, c_to, m_to);
+    c_to += cnt_before;
+    m_to += mass_before;
+    const u64 to = by_count ? (u64)c_to : m_to, from = to - (by_count ? (u64)bc : bm);
+    if (from < target && to >= target) s.list_hit = Hit{(uint32_t)t, c_to - bc, bc, m_to - bm};
+    __syncthreads();
+    const Hit h = s.list_hit;
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j)
+      if (t + j * kThreads < c && (uint32_t)((key[j] - lo) >> shift) == h.bin) s.list[atomicAdd(&s.n_list2, 1u)] = key[j];
+    __syncthreads();
+    c = (int)h.cnt;
+    cnt_before = h.cnt_before;
+    mass_before = h.mass_before;
+  }
+  c = min(c, kThreads);
+  const u64 key = sorted(s, s.list, c);
+  const u64 m = t < c ? mass_of(s, r, key_logit(key)) : 0ull;
+  const u64 to_m = mass_before + block_scan(s, m);
+  const u64 to = by_count ? (u64)cnt_before + t + 1 : to_m, from = by_count ? to - 1 : to - m;
+  if (t < c && from < target && to >= target)
+#pragma unroll
+    for (int q = 0; q < C; ++q) {
+      Smem* o = of_rank<C>(s, q);
+      o->res_idx = (int)(uint32_t)key;
+      o->res_mass = to_m;
+    }
+}
+
+// First token in order whose running count (by_count) or mass reaches the target; the row's bins
+// hold it.  Gives its index and the running mass up to and with it, in every CTA.
+template <int C>
+__device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u64 target) {
+  const int t = threadIdx.x;
+  find_bin<C>(s, by_count, target);
+  Hit h = s.hit;
+  const int bin = (int)h.bin;
+  u64 k0 = 0, k1 = ~0ull;                      // order keys of the tokens in question, inside the bin
+  const auto member = [&](float x, int i) {
+    if (bin_of(r, x) != bin) return false;
+    const u64 k = order_key(x, i);
+    return k >= k0 && k <= k1 && survives(s, r, x, bin);
+  };
+  // each level takes 9 bits off the span, so the sixth leaves fewer than a list holds
+  for (int level = 0; level < 8 && h.cnt > (uint32_t)kList; ++level) {
+    if (t == 0) {
+      s.key_min = ~0ull;
+      s.key_max = 0;
+    }
+    bins_clear(s.sub);
+    __syncthreads();
+    u64 lo = ~0ull, hi = 0;
+    each_logit(s, n, [&](float x, int i) {
+      if (member(x, base + i)) {
+        const u64 k = order_key(x, base + i);
+        lo = min(lo, k);
+        hi = max(hi, k);
+      }
+    });
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if ((t & 31) == 0) {
+      atomicMin(&s.key_min, lo);
+      atomicMax(&s.key_max, hi);
+    }
+    cluster_barrier<C>();
+    for (int q = 0; q < C; ++q) {
+      const Smem* o = of_rank<C>(s, q);
       lo = min(lo, o->key_min);
       hi = max(hi, o->key_max);
     }
-    cl.sync();
     k0 = lo;
     k1 = hi;
-    if (k0 == k1) {
-      // a run of equal logits: its m-th token in index order
-      const u64 w = mass_of(r, from_desc_key(k0)), need = target - (by_count ? (u64)cnt_before : mass_before);
-      u64 m = by_count ? need : (need + w - 1) / w;
-      if (m > cnt) m = cnt;
-      const int per = (n + kThreads - 1) / kThreads, i0 = min(n, t * per), i1 = min(n, i0 + per);
-      uint32_t mine = 0;
-      for (int i = i0; i < i1; ++i) mine += desc_key(s.x[i]) == k0;
-      const uint32_t incl = block_incl_scan<uint32_t>(mine, s.scan32);
-      if (t == kThreads - 1) s.eq_count = incl;
-      cl.sync();
-      uint32_t before = 0;
-      for (unsigned q = 0; q < cl.block_rank(); ++q) before += cl.map_shared_rank(&s, q)->eq_count;
-      const uint32_t excl = before + incl - mine;
-      if (excl < m && m <= (u64)excl + mine) {
-        uint32_t left = (uint32_t)m - excl;
-        int at = i0;
-        for (int i = i0; i < i1; ++i)
-          if (desc_key(s.x[i]) == k0 && --left == 0) at = i;
-        for (unsigned q = 0; q < cl.num_blocks(); ++q) {
-          Smem* o = cl.map_shared_rank(&s, q);
-          o->res_idx = base + at;
-          o->res_mass = mass_before + m * w;
-        }
-      }
-      cl.sync();
-      return;
+    const int shift = max(0, 64 - __clzll((long long)(k1 - k0)) - 9);
+    each_logit(s, n, [&](float x, int i) {
+      if (member(x, base + i)) bins_add(s.sub, (int)((order_key(x, base + i) - k0) >> shift), mass_of(s, r, x));
+    });
+    cluster_barrier<C>();
+    uint32_t c = 0;
+    u64 m = 0;
+    for (int q = 0; q < C; ++q) {
+      const Smem* o = of_rank<C>(s, q);
+      c += o->sub.cnt[t];
+      m += ((u64)o->sub.hi[t] << 32) + o->sub.lo[t];
     }
-    const int bits = 32 - __clz(k1 - k0), shift = max(0, bits - 10);
-    for (int i = t; i < n; i += kThreads)
-      if (member(s.x[i])) bins_add(s, (int)((desc_key(s.x[i]) - k0) >> shift), mass_of(r, s.x[i]));
-    uint32_t c, c_to;
-    u64 ms, m_to;
-    bins_sum(s, cl, c, ms, c_to, m_to);
-    const u64 to = by_count ? (u64)cnt_before + c_to : mass_before + m_to, from = to - (by_count ? (u64)c : ms);
-    if (from < target && to >= target) {
-      s.key_min = k0 + ((uint32_t)t << shift);
-      s.hit_cnt_before = cnt_before + c_to - c;
-      s.hit_cnt = c;
-      s.hit_mass_before = mass_before + m_to - ms;
-    }
-    __syncthreads();
-    k0 = s.key_min;
-    k1 = min(k1, k0 + ((1u << shift) - 1u));
+    uint32_t c_to = c;
+    u64 m_to = m;
+    block_scan(s, c_to, m_to);
+    c_to += h.cnt_before;
+    m_to += h.mass_before;
+    const u64 to = by_count ? (u64)c_to : m_to, from = to - (by_count ? (u64)c : m);
+    if (from < target && to >= target) s.hit = Hit{(uint32_t)t, c_to - c, c, m_to - m};   // the same in every CTA
+    cluster_barrier<C>();
+    h = s.hit;
+    k0 += (u64)h.bin << shift;
+    k1 = min(k1, k0 + ((1ull << shift) - 1ull));
   }
+  gather<C>(s, base, n, member);
+  if (my_rank<C>() == 0) {
+    resolve_list<C>(s, r, (int)min(h.cnt, (uint32_t)kList), h.cnt_before, h.mass_before, by_count, target);
+    if (t == 0) s.n_list = 0;
+  }
+  cluster_barrier<C>();
 }
 
+// 16-byte loads of the slice where the row allows it, single ones else.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) k_sample(const __grid_constant__ Params p) {
+__device__ __forceinline__ float load_slice(Smem& s, const T* src, int n) {
+  constexpr int V = 16 / sizeof(T);
+  float mx = -INFINITY;
+  const auto put = [&](float x, int i) {
+    x += 0.f;                                  // -0 counts as 0
+    if (!(x == x)) x = -INFINITY;              // NaN is never drawn
+    s.x[i] = x;
+    mx = fmaxf(mx, x);
+  };
+  const int nv = (reinterpret_cast<uintptr_t>(src) & 15) ? 0 : n / V;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nv; i += kThreads) {
+    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(src) + i);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float x[V];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (V == 4) {
+        x[j] = __uint_as_float(w[j]);
+      } else {
+        const float2 f = ops::Elem<T>::unpack(w[j]);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      x[j] += 0.f;
+      if (!(x[j] == x[j])) x[j] = -INFINITY;
+      mx = fmaxf(mx, x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(&s.x[i * V + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+  }
+  for (int i = nv * V + threadIdx.x; i < n; i += kThreads) put(ops::Elem<T>::to_f32(src[i]), i);
+  if (threadIdx.x < 4 && (n + (int)threadIdx.x) < ((n + 3) & ~3)) s.x[n + threadIdx.x] = -INFINITY;
+  return mx;
+}
+
+template <typename T, int C>
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) unsigned char raw[];
   Smem& s = *reinterpret_cast<Smem*>(raw);
-  cg::cluster_group cl = cg::this_cluster();
   const int t = threadIdx.x;
-  const long long row = blockIdx.x / cl.num_blocks();
-  const int base = (int)cl.block_rank() * p.slice, n = max(0, min(p.slice, p.n - base));
+  const long long row = blockIdx.x / C;
+  const int rank = my_rank<C>(), base = rank * p.slice, n = max(0, min(p.slice, p.n - base));
+  if (t < 64) s.exp2_tab[t] = kExp2[t];
+  bins_clear(s.bins);
+  if (t == 0) s.n_list = 0;
+  if constexpr (C > 1) cg::this_cluster().barrier_arrive();
   griddep_launch();
   griddep_wait();
 
-  // ---- the slice and the row's maximum (NaN as -inf, -0 as 0)
-  const T* src = (const T*)p.logits + row * p.stride + base;
-  float mx = -INFINITY;
-  for (int i = t; i < n; i += kThreads) {
-    float x = ops::Elem<T>::to_f32(src[i]) + 0.f;
-    if (!(x == x)) x = -INFINITY;
-    s.x[i] = x;
-    mx = fmaxf(mx, x);
-  }
-  mx = warp_max(mx);
+  // ---- the slice and the row's maximum
+  float mx = warp_max(load_slice<T>(s, (const T*)p.logits + row * p.stride + base, n));
   if ((t & 31) == 0) s.red[t >> 5] = mx;
-  bins_clear(s);
   __syncthreads();
-  if (t < 32) {
-    mx = warp_max(s.red[t]);
-    if (t == 0) s.cta_max = mx;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) mx = fmaxf(mx, s.red[i]);
+  if constexpr (C > 1) {
+    cg::this_cluster().barrier_wait();         // every CTA runs, so that its memory may be written
+    if (t < C) of_rank<C>(s, t)->max_of[rank] = mx;
+    cluster_barrier<C>();
+#pragma unroll
+    for (int q = 0; q < C; ++q) mx = fmaxf(mx, s.max_of[q]);
   }
-  cl.sync();
-  for (unsigned q = 0; q < cl.num_blocks(); ++q) mx = fmaxf(mx, cl.map_shared_rank(&s, q)->cta_max);
 
+  if (mx == INFINITY) {    // the infinite ones share the draw: as logits 0 among -inf
+    for (int i = t; i < n; i += kThreads) s.x[i] = s.x[i] == INFINITY ? 0.f : -INFINITY;
+    mx = 0.f;
+    __syncthreads();
+  }
   Row r;
   double temp = p.temperature ? (double)p.temperature[row] : p.temperature1;
   int k = p.top_k ? p.top_k[row] : p.top_k1;
   const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p1;
+  const double min_p = fmin(1.0, p.min_p ? (double)p.min_p[row] : p.min_p1);
   const double u = p.u[row];
   if (!(temp > 0.0)) {   // greedy
     temp = 1.0;
     k = 1;
   }
   r.mx = mx;
-  r.inv_t = 1.0 / temp;
-  r.min_p = fmin(1.0, p.min_p ? (double)p.min_p[row] : p.min_p1);
+  r.mxd = (double)mx;
+  r.c64 = 64.0 * 1.4426950408889634 / temp;
+  r.min_p44 = min_p * 17592186044416.0;
   r.c = (float)(1.4426950408889634 / temp);
   r.cut_log2 = kRangeLog2;
-  if (r.min_p > 0.0) r.cut_log2 = fminf(kRangeLog2, (float)-log2(r.min_p) * 1.0001f + 0.001f);
+  if (min_p > 0.0) r.cut_log2 = fminf(kRangeLog2, (float)-log2(min_p) * 1.0001f + 0.001f);
   r.bin_scale = (float)kBins / r.cut_log2;
+  r.sure = (int)(((r.cut_log2 - 0.001f) * 0.9998f - 0.002f) * r.bin_scale);
   if (mx == -INFINITY) {   // nothing to draw from
-    cl.sync();
-    if (cl.block_rank() == 0 && t == 0) p.out[row] = -1;
+    if (rank == 0 && t == 0) p.out[row] = -1;
     return;
   }
-
-  // ---- bins of the row
-  for (int i = t; i < n; i += kThreads) {
-    const float x = s.x[i];
-    const int b = bin_of(r, x);
-    if (b >= 0) {
-      const u64 m = mass_of(r, x);
-      if (m) bins_add(s, b, m);
-    }
-  }
-  {
-    uint32_t c, c_to;
-    u64 m, m_to;
-    bins_sum(s, cl, c, m, c_to, m_to);
-    s.cnt_to[t] = c_to;
-    s.mass_to[t] = m_to;
-  }
-  __syncthreads();
-  const uint32_t total = s.cnt_to[kBins - 1];
-  u64 kept = s.mass_to[kBins - 1];
-  const bool cut_k = k > 0 && (uint32_t)k < total, cut_p = top_p < 1.0;
   const auto reach = [](double share, u64 of) {   // the whole-number mass that `share` of `of` asks for
     if (!(share > 0.0)) return (u64)1;
     const u64 v = (u64)ceil(share * (double)of);
     return v < 1 ? (u64)1 : v > of ? of : v;
   };
 
-  // ---- the head that decides: up to the bin of the k-th token, of the top-p mass, or of the draw
-  const u64 target0 = cut_k ? (u64)k : reach(cut_p ? top_p : u, kept);
-  {
-    const u64 to = cut_k ? (u64)s.cnt_to[t] : s.mass_to[t], from = t ? (cut_k ? (u64)s.cnt_to[t - 1] : s.mass_to[t - 1]) : 0ull;
-    if (from < target0 && to >= target0) s.hit_bin = t;
-  }
-  __syncthreads();
-  const int last = s.hit_bin;
-  const int head = (int)s.cnt_to[last];
-  __syncthreads();
-  if (head <= kList) {
-    gather(s, cl, base, n, [&](float x) {
+  // ---- the head that decides: up to the bin of the k-th token (from counts alone), of the top-p
+  // mass, or of the draw
+  bool cut_k = k > 0 && k < p.n;
+  const bool cut_p = top_p < 1.0;
+  uint32_t total;
+  u64 kept;
+  int head = 0x7fffffff;
+  if (cut_k && k <= kHead) {
+    each_logit(s, n, [&](float x, int) {
       const int b = bin_of(r, x);
-      return b >= 0 && b <= last && mass_of(r, x) > 0;
+      if (b >= 0) atomicAdd(&s.bins.cnt[b], 1u);
     });
-    if (cl.block_rank() == 0) {
-      sort_list(s, head);
-      u64 m0 = 0, m1 = 0;
-      if (2 * t < head) m0 = mass_of(r, from_desc_key((uint32_t)(s.list[2 * t] >> 32)));
-      if (2 * t + 1 < head) m1 = mass_of(r, from_desc_key((uint32_t)(s.list[2 * t + 1] >> 32)));
-      const u64 to1 = block_incl_scan<u64>(m0 + m1, s.scan64), to0 = to1 - m1, from0 = to0 - m0;
-      if (cut_k) {
-        if (k - 1 == 2 * t) s.res_mass = to0;
-        if (k - 1 == 2 * t + 1) s.res_mass = to1;
+    sum_bins<C>(s, total, kept);
+    if (total <= (uint32_t)kHead) {
+      head = (int)total;
+      if (t == 0) s.hit.bin = kBins - 1;
+      __syncthreads();
+    } else {
+      find_bin<C>(s, true, (u64)k);           // total > kHead >= k: it is there
+      head = (int)(s.hit.cnt_before + s.hit.cnt);
+    }
+    if (head > kHead) {                        // many equal or near-equal logits around the k-th
+      cluster_barrier<C>();
+      bins_clear(s.bins);
+      __syncthreads();
+    }
+  }
+  if (head > kHead) {
+    each_logit(s, n, [&](float x, int) {
+      const int b = bin_of(r, x);
+      const u64 m = mass_of(s, r, x, b);
+      if (b >= 0 && m) bins_add(s.bins, b, m);
+    });
+    sum_bins<C>(s, total, kept);
+    cut_k = cut_k && (uint32_t)k < total;
+    find_bin<C>(s, cut_k, cut_k ? (u64)k : reach(cut_p ? top_p : u, kept));
+    head = (int)(s.hit.cnt_before + s.hit.cnt);
+  }
+  if (head <= kHead) {
+    const int last = (int)s.hit.bin;
+    gather<C>(s, base, n, [&](float x, int) {
+      const int b = bin_of(r, x);
+      return b >= 0 && b <= last && survives(s, r, x, b);
+    });
+    if (rank == 0) {
+      const int c = (int)s.n_list;             // exact survivors: at most `head`
+      const u64 key = sorted(s, s.list, c);
+      const u64 m = t < c ? mass_of(s, r, key_logit(key)) : 0ull;
+      const u64 to = block_scan(s, m), from = to - m;
+      if (cut_k || last == kBins - 1) {        // the list holds all that is left
+        if (t == min(c, cut_k ? k : c) - 1) s.res_mass = to;
         __syncthreads();
         kept = s.res_mass;
         __syncthreads();
       }
       if (cut_p) {
         const u64 g = reach(top_p, kept);
-        if (from0 < g && to0 >= g) s.res_mass = to0;
-        if (to0 < g && to1 >= g) s.res_mass = to1;
+        if (from < g && to >= g) s.res_mass = to;
         __syncthreads();
         kept = s.res_mass;
         __syncthreads();
       }
       const u64 g = reach(u, kept);
-      if (from0 < g && to0 >= g) p.out[row] = (int32_t)(uint32_t)s.list[2 * t];
-      if (to0 < g && to1 >= g) p.out[row] = (int32_t)(uint32_t)s.list[2 * t + 1];
+      if (from < g && to >= g) p.out[row] = (int32_t)(uint32_t)key;
     }
     return;
   }
   if (cut_k) {
-    select(s, cl, r, base, n, true, (u64)k);
+    select<C>(s, r, base, n, true, (u64)k);
     kept = s.res_mass;
   }
   if (cut_p) {
-    select(s, cl, r, base, n, false, reach(top_p, kept));
+    select<C>(s, r, base, n, false, reach(top_p, kept));
     kept = s.res_mass;
   }
-  select(s, cl, r, base, n, false, reach(u, kept));
-  if (cl.block_rank() == 0 && t == 0) p.out[row] = s.res_idx;
+  select<C>(s, r, base, n, false, reach(u, kept));
+  if (rank == 0 && t == 0) p.out[row] = s.res_idx;
 }
 
 }  // namespace sample

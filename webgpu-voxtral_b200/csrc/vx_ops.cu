@@ -267,13 +267,18 @@ cudaError_t launch_attention(pattn::Params p, const vx_kv_pages& c, const Plan& 
 }
 
 // ------------------------------------------------------------------ sampling
-template <typename T>
-cudaError_t launch_sample(const sample::Params& p, int rows, int cluster, cudaStream_t s) {
+template <typename T, int C>
+cudaError_t launch_sample(const sample::Params& p, int rows, cudaStream_t s) {
   static std::atomic<int> done[kMaxDevices];
   const size_t bytes = sizeof(sample::Smem) + (size_t)p.slice * 4;
-  cudaError_t ce = allow_smem(sample::k_sample<T>, done, sizeof(sample::Smem) + sample::kMaxSlice * 4);
+  cudaError_t ce = allow_smem(sample::k_sample<T, C>, done, sizeof(sample::Smem) + sample::kMaxSlice * 4);
   if (ce != cudaSuccess) return ce;
-  return launch_cluster(cluster, sample::k_sample<T>, dim3((unsigned)rows * cluster), dim3(sample::kThreads), bytes, s, p);
+  return launch_cluster(C, sample::k_sample<T, C>, dim3((unsigned)rows * C), dim3(sample::kThreads), bytes, s, p);
+}
+template <typename T>
+cudaError_t launch_sample(const sample::Params& p, int rows, int cluster, cudaStream_t s) {
+  return cluster == 1 ? launch_sample<T, 1>(p, rows, s) : cluster == 2 ? launch_sample<T, 2>(p, rows, s)
+         : cluster == 4 ? launch_sample<T, 4>(p, rows, s) : launch_sample<T, 8>(p, rows, s);
 }
 
 }  // namespace
@@ -384,18 +389,16 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   if (reinterpret_cast<uintptr_t>(a.logits) % elem_size(a.dtype)) return e.fail(VX_E_INVALID, "logits must be aligned to their type");
   const int sms = sm_count();
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
+  // CTAs a row: slices of at most 16384 logits, so that two CTAs share an SM
   int cluster = 1;
-  while (cluster < sample::kMaxCluster &&
-         ((a.n_cols + cluster - 1) / cluster > sample::kMaxSlice ||
-          ((long long)a.n_rows * cluster * 2 <= sms && (a.n_cols + cluster - 1) / cluster > 4096)))
-    cluster *= 2;
+  while (cluster < sample::kMaxCluster && (a.n_cols + cluster - 1) / cluster > 16384) cluster *= 2;
   if ((long long)a.n_rows * cluster > 0x7fffffff) return e.fail(VX_E_RANGE, "%d rows are too many for one call", a.n_rows);
   sample::Params p{};
   p.logits = a.logits; p.stride = a.row_stride; p.u = a.u;
   p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.top_k = a.top_k;
   p.temperature1 = a.temperature_all; p.top_p1 = a.top_p_all; p.min_p1 = a.min_p_all; p.top_k1 = a.top_k_all;
   p.out = a.out; p.n = a.n_cols;
-  p.slice = (a.n_cols + cluster - 1) / cluster;
+  p.slice = ((a.n_cols + cluster - 1) / cluster + 7) & ~7;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t ce = a.dtype == 0 ? launch_sample<__half>(p, a.n_rows, cluster, s)
                          : a.dtype == 1 ? launch_sample<__nv_bfloat16>(p, a.n_rows, cluster, s) : launch_sample<float>(p, a.n_rows, cluster, s);
