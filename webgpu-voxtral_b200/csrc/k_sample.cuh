@@ -14,17 +14,24 @@
 // boundaries by 2^-24, which at 131072 tokens of about equal weight changes one draw in a
 // hundred.
 //
-// No sort of the row.  The row lies in the shared memory of a cluster of 1 to 8 CTAs.  One pass
-// puts each survivor's count and mass into one of 2048 bins, linear in log w; running sums over
-// the bins (each CTA sums a share of them over the cluster) find the bin in which a count or mass
-// is reached.  Where the whole head up to that bin is at most 512 tokens it is gathered into one
+// No sort of the row.  A cluster of 1 to 8 CTAs shares a row (kept in shared memory where the
+// slices are small, read again from L2 where not).  After the pass for the maximum, one pass puts
+// each survivor's count and mass into one of 2048 bins, linear in the logit; running sums over the
+// bins (each CTA sums a share of them over the cluster) find the bin in which a count or mass is
+// reached.  Where the whole head up to that bin is at most 512 tokens it is gathered into one
 // CTA, sorted exactly, and all three limits are found in the sorted list; with top-k that head is
 // found from counts alone, so only its tokens need an exponential.  Otherwise the tokens of the
 // bin in question are gathered, binned again by their order key (logit, then index) and the few of
 // one such bin sorted.  A bin of more than 1024 tokens is first binned again over the cluster by the
 // same key; runs of equal logits need nothing of their own, as their keys differ in the index.
+//
+// Bound: not HBM (200 rows of 131072 f32 logits would take 16 us) but the pass of the masses, about
+// 45 instructions and two or three shared-memory atomics a logit.  One B200: those 200 rows 143 us
+// with top-p 0.95, 67 us with top-k 50; 64 rows of 131072 bf16 logits with all filters 35 us.
 #pragma once
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "vx_ops.cuh"
 
@@ -40,7 +47,8 @@ constexpr int kSub = kThreads;         // second-level bins, one a thread
 constexpr int kHead = kThreads;        // tokens sorted at once, one a thread
 constexpr int kList = 1024;            // tokens gathered at once
 constexpr int kFew = 96;               // tokens of a list that are sorted rather than binned again
-constexpr int kMaxSlice = 32768;       // logits a CTA holds
+constexpr int kMaxCols = 262144;
+constexpr int kResident = 16384;       // logits that a CTA keeps in shared memory, at most
 constexpr int kMaxCluster = 8;
 constexpr float kRangeLog2 = 45.f;     // w below 2^-45 rounds to mass 0
 
@@ -54,6 +62,7 @@ struct Params {
   int top_k1;
   int32_t* out;
   int n, slice;
+  int resident;   // the slice is kept in shared memory
 };
 
 // Where a running count or mass reaches a target.
@@ -72,8 +81,8 @@ struct Smem {
   double exp2_tab[64];                 // 2^(j / 64)
   u64 scan64[16];
   uint32_t scan32[16];
-  float red[16];
-  float max_of[kMaxCluster];           // each CTA's, and the totals of each one's share of bins
+  float2 red[16];
+  float2 range_of[kMaxCluster];        // each CTA's largest and smallest, and the totals of each one's share of bins
   uint32_t tot_cnt[kMaxCluster];
   u64 tot_mass[kMaxCluster];
   u64 key_min, key_max;
@@ -158,7 +167,7 @@ __device__ __forceinline__ int my_rank() {
 }
 
 struct Row {
-  float mx, c, bin_scale, cut_log2;    // log2 w = -(mx - x) c; nothing below -cut_log2 survives
+  float mx, cut, scale;                // bin (mx - x) * scale; nothing further than cut below mx survives
   int sure;                            // every logit of the bins below this one survives
   double mxd, c64, min_p44;            // 64 log2(e) / T; min_p 2^44
 };
@@ -207,8 +216,17 @@ __device__ __forceinline__ u64 mass_of(const Smem& s, const Row& r, float x, int
 __device__ __forceinline__ u64 mass_of(const Smem& s, const Row& r, float x) { return whole(weight44(s, r, x)); }
 // Bin of a logit, -1 for one that cannot survive (the exact test is mass_of's).
 __device__ __forceinline__ int bin_of(const Row& r, float x) {
-  const float t = (r.mx - x) * r.c;
-  return t <= r.cut_log2 ? min(kBins - 1, (int)(t * r.bin_scale)) : -1;
+  const float d = r.mx - x;
+  return d <= r.cut ? (int)(d * r.scale) : -1;
+}
+// Smallest distance from the maximum that falls into bin b or a later one.
+__device__ __forceinline__ float bin_edge(const Row& r, int b) {
+  if (b <= 0) return 0.f;
+  if (b >= kBins) return INFINITY;
+  float d = (float)b / r.scale;
+  for (int i = 0; i < 4 && d > 0.f && __uint_as_float(__float_as_uint(d) - 1) * r.scale >= (float)b; ++i) d = __uint_as_float(__float_as_uint(d) - 1);
+  for (int i = 0; i < 4 && d * r.scale < (float)b; ++i) d = __uint_as_float(__float_as_uint(d) + 1);
+  return d;
 }
 // Whether a logit of bin b survives.
 __device__ __forceinline__ bool survives(const Smem& s, const Row& r, float x, int b) {
@@ -323,34 +341,97 @@ __device__ void find_bin(Smem& s, bool by_count, u64 target) {
   cluster_barrier<C>();
 }
 
-// Calls f(x, i) for every logit of the slice, four at a time (the slice ends in -inf).
-template <typename F>
-__device__ __forceinline__ void each_logit(const Smem& s, int n, F f) {
-#pragma unroll 2
-  for (int v = threadIdx.x; v * 4 < n; v += kThreads) {
-    const float4 x = *reinterpret_cast<const float4*>(&s.x[4 * v]);
-    f(x.x, 4 * v);
-    f(x.y, 4 * v + 1);
-    f(x.z, 4 * v + 2);
-    f(x.w, 4 * v + 3);
+// The CTA's slice of the row: in shared memory, or read again from global memory (L2) each time.
+template <typename T>
+struct Slice {
+  const T* g;
+  int n;
+  bool resident, wide;                 // wide: four logits in one load
+  bool inf;                            // the row holds +inf: those draw as logits 0, the others not at all
+};
+__device__ __forceinline__ float clean(float x) {
+  x += 0.f;                            // -0 counts as 0
+  return x == x ? x : -INFINITY;       // NaN is never drawn
+}
+// Calls f(x, i) for the logits of the slice, x[0..3] at i (-inf past the end).  Four loads a thread are
+// on their way before the first is used: neither the branches of a ragged end nor what f does to
+// shared memory stand between them.
+template <typename T, bool FIRST, typename F>
+__device__ __forceinline__ void each_four(const Smem& s, const Slice<T>& sl, F f) {
+  constexpr int U = 4, STEP = 4 * kThreads;
+  for (int i0 = 4 * threadIdx.x; i0 < sl.n; i0 += U * STEP) {
+    float x[U][4];
+    const bool all = i0 + (U - 1) * STEP + 4 <= sl.n;
+    if (!FIRST && sl.resident) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // past the end: the last four again, not used
+        const float4 q = *reinterpret_cast<const float4*>(&s.x[min(i0 + u * STEP, (sl.n - 1) & ~3)]);
+        x[u][0] = q.x; x[u][1] = q.y; x[u][2] = q.z; x[u][3] = q.w;
+      }
+    } else {
+      if (sl.wide && all) {
+        typedef typename std::conditional<sizeof(T) == 4, float4, uint2>::type Four;
+        Four q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = __ldg(reinterpret_cast<const Four*>(sl.g + i0 + u * STEP));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if constexpr (sizeof(T) == 4) {
+            x[u][0] = q[u].x; x[u][1] = q[u].y; x[u][2] = q[u].z; x[u][3] = q[u].w;
+          } else {
+            const float2 a = ops::Elem<T>::unpack(q[u].x), b = ops::Elem<T>::unpack(q[u].y);
+            x[u][0] = a.x; x[u][1] = a.y; x[u][2] = b.x; x[u][3] = b.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[u][j] = i0 + u * STEP + j < sl.n ? ops::Elem<T>::to_f32(sl.g[i0 + u * STEP + j]) : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = clean(x[u][j]);
+      if (!FIRST && sl.inf)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[u][j] = x[u][j] == INFINITY ? 0.f : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (all || i0 + u * STEP < sl.n) f(x[u], i0 + u * STEP);
   }
 }
 
-// Puts the cluster's tokens for which `take(x, i)` holds into the list of CTA 0, whose n_list is 0:
-// first into a list of the CTA's own, then those together.
-template <int C, typename F>
-__device__ __forceinline__ void gather(Smem& s, int base, int n, F take) {
+// Puts the cluster's tokens of the bins [bin0, bin1] whose order keys are in [k0, k1] into the list of
+// CTA 0, whose n_list is 0: first into a list of the CTA's own, then those together.
+template <typename T, int C>
+__device__ __forceinline__ void gather(Smem& s, const Row& r, const Slice<T>& sl, int base, int bin0, int bin1, u64 k0, u64 k1) {
   if constexpr (C > 1) {
     if (threadIdx.x == 0) s.n_own = 0;
     __syncthreads();
   }
   uint32_t* count = C > 1 ? &s.n_own : &s.n_list;
   u64* list = C > 1 ? s.list2 : s.list;
-  each_logit(s, n, [&](float x, int i) {
-    if (take(x, base + i)) {
-      const uint32_t at = atomicAdd(count, 1u);
-      if (at < (uint32_t)kList) list[at] = order_key(x, base + i);
-    }
+  // the bins as a range [d0, d1) of distances from the maximum; the exact tests where they may matter
+  const float d0 = bin_edge(r, bin0), d1 = fminf(bin_edge(r, bin1 + 1), nextafterf(r.cut, INFINITY));
+  const bool keys = k0 > 0 || k1 < ~0ull, border = bin1 >= r.sure;
+  each_four<T, false>(s, sl, [&](const float (&x)[4], int i) {
+    float d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = r.mx - x[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (d[j] >= d0 && d[j] < d1) {
+        const u64 k = order_key(x[j], base + i + j);
+        if (keys && (k < k0 || k > k1)) continue;
+        if (border && !survives(s, r, x[j], bin_of(r, x[j]))) continue;
+        const uint32_t at = atomicAdd(count, 1u);
+        if (at < (uint32_t)kList) list[at] = k;
+      }
   });
   if constexpr (C > 1) {
     __syncthreads();
@@ -463,8 +544,12 @@ __device__ void resolve_list(Smem& s, const Row& r, int c, uint32_t cnt_before, 
 
 // First token in order whose running count (by_count) or mass reaches the target; the row's bins
 // hold it.  Gives its index and the running mass up to and with it, in every CTA.
-template <int C>
-__device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u64 target) {
+// Arguments by value, and shared memory by its own name: what is reached through a reference is read
+// again after every store.
+template <typename T, int C>
+__device__ __noinline__ void select(const Row r, const Slice<T> sl, int base, bool by_count, u64 target) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  Smem& s = *reinterpret_cast<Smem*>(raw);
   const int t = threadIdx.x;
   find_bin<C>(s, by_count, target);
   Hit h = s.hit;
@@ -484,12 +569,14 @@ __device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u6
     bins_clear(s.sub);
     __syncthreads();
     u64 lo = ~0ull, hi = 0;
-    each_logit(s, n, [&](float x, int i) {
-      if (member(x, base + i)) {
-        const u64 k = order_key(x, base + i);
-        lo = min(lo, k);
-        hi = max(hi, k);
-      }
+    each_four<T, false>(s, sl, [&](const float (&x)[4], int i) {
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j)
+        if (member(x[j], base + i + j)) {
+          const u64 k = order_key(x[j], base + i + j);
+          lo = min(lo, k);
+          hi = max(hi, k);
+        }
     });
     for (int o = 16; o > 0; o >>= 1) {
       lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -508,8 +595,10 @@ __device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u6
     k0 = lo;
     k1 = hi;
     const int shift = max(0, 64 - __clzll((long long)(k1 - k0)) - 9);
-    each_logit(s, n, [&](float x, int i) {
-      if (member(x, base + i)) bins_add(s.sub, (int)((order_key(x, base + i) - k0) >> shift), mass_of(s, r, x));
+    each_four<T, false>(s, sl, [&](const float (&x)[4], int i) {
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j)
+        if (member(x[j], base + i + j)) bins_add(s.sub, (int)((order_key(x[j], base + i + j) - k0) >> shift), mass_of(s, r, x[j]));
     });
     cluster_barrier<C>();
     uint32_t c = 0;
@@ -531,7 +620,7 @@ __device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u6
     k0 += (u64)h.bin << shift;
     k1 = min(k1, k0 + ((1ull << shift) - 1ull));
   }
-  gather<C>(s, base, n, member);
+  gather<T, C>(s, r, sl, base, bin, bin, k0, k1);
   if (my_rank<C>() == 0) {
     resolve_list<C>(s, r, (int)min(h.cnt, (uint32_t)kList), h.cnt_before, h.mass_before, by_count, target);
     if (t == 0) s.n_list = 0;
@@ -539,45 +628,19 @@ __device__ void select(Smem& s, const Row& r, int base, int n, bool by_count, u6
   cluster_barrier<C>();
 }
 
-// 16-byte loads of the slice where the row allows it, single ones else.
+// Largest and smallest finite logit of the slice; fills the resident copy.
 template <typename T>
-__device__ __forceinline__ float load_slice(Smem& s, const T* src, int n) {
-  constexpr int V = 16 / sizeof(T);
-  float mx = -INFINITY;
-  const auto put = [&](float x, int i) {
-    x += 0.f;                                  // -0 counts as 0
-    if (!(x == x)) x = -INFINITY;              // NaN is never drawn
-    s.x[i] = x;
-    mx = fmaxf(mx, x);
-  };
-  const int nv = (reinterpret_cast<uintptr_t>(src) & 15) ? 0 : n / V;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nv; i += kThreads) {
-    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(src) + i);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    float x[V];
+__device__ __forceinline__ void scan_slice(Smem& s, const Slice<T>& sl, float& mx, float& mn) {
+  mx = -INFINITY;
+  mn = INFINITY;
+  each_four<T, true>(s, sl, [&](const float (&x)[4], int i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (V == 4) {
-        x[j] = __uint_as_float(w[j]);
-      } else {
-        const float2 f = ops::Elem<T>::unpack(w[j]);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      x[j] += 0.f;
-      if (!(x[j] == x[j])) x[j] = -INFINITY;
       mx = fmaxf(mx, x[j]);
+      mn = fminf(mn, x[j] == -INFINITY ? INFINITY : x[j]);
     }
-#pragma unroll
-    for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(&s.x[i * V + j]) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-  }
-  for (int i = nv * V + threadIdx.x; i < n; i += kThreads) put(ops::Elem<T>::to_f32(src[i]), i);
-  if (threadIdx.x < 4 && (n + (int)threadIdx.x) < ((n + 3) & ~3)) s.x[n + threadIdx.x] = -INFINITY;
-  return mx;
+    if (sl.resident) *reinterpret_cast<float4*>(&s.x[i]) = make_float4(x[0], x[1], x[2], x[3]);
+  });
 }
 
 template <typename T, int C>
@@ -586,7 +649,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   Smem& s = *reinterpret_cast<Smem*>(raw);
   const int t = threadIdx.x;
   const long long row = blockIdx.x / C;
-  const int rank = my_rank<C>(), base = rank * p.slice, n = max(0, min(p.slice, p.n - base));
+  const int rank = my_rank<C>(), base = rank * p.slice;
+  Slice<T> sl;
+  sl.g = (const T*)p.logits + row * p.stride + base;
+  sl.n = max(0, min(p.slice, p.n - base));
+  sl.resident = p.resident;
+  sl.wide = reinterpret_cast<uintptr_t>(sl.g) % (4 * sizeof(T)) == 0;
+  sl.inf = false;
   if (t < 64) s.exp2_tab[t] = kExp2[t];
   bins_clear(s.bins);
   if (t == 0) s.n_list = 0;
@@ -594,25 +663,40 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   griddep_launch();
   griddep_wait();
 
-  // ---- the slice and the row's maximum
-  float mx = warp_max(load_slice<T>(s, (const T*)p.logits + row * p.stride + base, n));
-  if ((t & 31) == 0) s.red[t >> 5] = mx;
+  // ---- the row's largest and smallest logit
+  float mx, mn;
+  scan_slice(s, sl, mx, mn);
+  mx = warp_max(mx);
+  mn = -warp_max(-mn);
+  if ((t & 31) == 0) s.red[t >> 5] = make_float2(mx, mn);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) mx = fmaxf(mx, s.red[i]);
+  for (int i = 0; i < kThreads / 32; ++i) {
+    mx = fmaxf(mx, s.red[i].x);
+    mn = fminf(mn, s.red[i].y);
+  }
   if constexpr (C > 1) {
     cg::this_cluster().barrier_wait();         // every CTA runs, so that its memory may be written
-    if (t < C) of_rank<C>(s, t)->max_of[rank] = mx;
+    if (t < C) of_rank<C>(s, t)->range_of[rank] = make_float2(mx, mn);
     cluster_barrier<C>();
 #pragma unroll
-    for (int q = 0; q < C; ++q) mx = fmaxf(mx, s.max_of[q]);
+    for (int q = 0; q < C; ++q) {
+      mx = fmaxf(mx, s.range_of[q].x);
+      mn = fminf(mn, s.range_of[q].y);
+    }
   }
-
-  if (mx == INFINITY) {    // the infinite ones share the draw: as logits 0 among -inf
-    for (int i = t; i < n; i += kThreads) s.x[i] = s.x[i] == INFINITY ? 0.f : -INFINITY;
-    mx = 0.f;
+  if (mx == -INFINITY) {   // nothing to draw from
+    if (rank == 0 && t == 0) p.out[row] = -1;
+    return;
+  }
+  if (mx == INFINITY) {
+    sl.inf = true;
+    mx = mn = 0.f;
+    if (sl.resident)
+      for (int i = t; i < sl.n; i += kThreads) s.x[i] = s.x[i] == INFINITY ? 0.f : -INFINITY;
     __syncthreads();
   }
+
   Row r;
   double temp = p.temperature ? (double)p.temperature[row] : p.temperature1;
   int k = p.top_k ? p.top_k[row] : p.top_k1;
@@ -623,19 +707,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     temp = 1.0;
     k = 1;
   }
+  temp = fmin(fmax(temp, 1e-250), 1e30);       // past these the draw is greedy, or uniform, already
   r.mx = mx;
   r.mxd = (double)mx;
   r.c64 = 64.0 * 1.4426950408889634 / temp;
   r.min_p44 = min_p * 17592186044416.0;
-  r.c = (float)(1.4426950408889634 / temp);
-  r.cut_log2 = kRangeLog2;
-  if (min_p > 0.0) r.cut_log2 = fminf(kRangeLog2, (float)-log2(min_p) * 1.0001f + 0.001f);
-  r.bin_scale = (float)kBins / r.cut_log2;
-  r.sure = (int)(((r.cut_log2 - 0.001f) * 0.9998f - 0.002f) * r.bin_scale);
-  if (mx == -INFINITY) {   // nothing to draw from
-    if (rank == 0 && t == 0) p.out[row] = -1;
-    return;
-  }
+  // how far below the maximum a logit can survive: until its mass rounds to 0, or to min-p; and at
+  // least to 0.999 of that, so that the bins there need no exact test
+  const double to_logit = temp * 0.6931471805599453;
+  const double far = min_p > 0.0 ? fmin(-log2(min_p), (double)kRangeLog2) : (double)kRangeLog2;
+  const float span = fmaxf(mx - mn, 1e-30f);                   // bins need not reach past the smallest
+  r.cut = fminf((float)(far * to_logit * 1.001 + 1e-6 * to_logit), span);
+  r.scale = (float)(kBins - 1) / r.cut;
+  const float sure = fminf((float)(far * to_logit * 0.999), span) * r.scale;
+  r.sure = sure < (float)(kBins - 1) ? (int)sure : mx - mn < (float)(far * to_logit * 0.999) ? kBins : kBins - 1;
   const auto reach = [](double share, u64 of) {   // the whole-number mass that `share` of `of` asks for
     if (!(share > 0.0)) return (u64)1;
     const u64 v = (u64)ceil(share * (double)of);
@@ -650,9 +735,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   u64 kept;
   int head = 0x7fffffff;
   if (cut_k && k <= kHead) {
-    each_logit(s, n, [&](float x, int) {
-      const int b = bin_of(r, x);
-      if (b >= 0) atomicAdd(&s.bins.cnt[b], 1u);
+    each_four<T, false>(s, sl, [&](const float (&x)[4], int) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b = bin_of(r, x[j]);
+        if (b >= 0) atomicAdd(&s.bins.cnt[b], 1u);
+      }
     });
     sum_bins<C>(s, total, kept);
     if (total <= (uint32_t)kHead) {
@@ -670,10 +758,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     }
   }
   if (head > kHead) {
-    each_logit(s, n, [&](float x, int) {
-      const int b = bin_of(r, x);
-      const u64 m = mass_of(s, r, x, b);
-      if (b >= 0 && m) bins_add(s.bins, b, m);
+    each_four<T, false>(s, sl, [&](const float (&x)[4], int) {
+      int b[4];
+      double w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = bin_of(r, x[j]);
+        w[j] = weight44(s, r, x[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 m = b[j] < r.sure || w[j] >= r.min_p44 ? whole(w[j]) : 0ull;
+        if (b[j] >= 0 && m) bins_add(s.bins, b[j], m);
+      }
     });
     sum_bins<C>(s, total, kept);
     cut_k = cut_k && (uint32_t)k < total;
@@ -682,10 +779,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   }
   if (head <= kHead) {
     const int last = (int)s.hit.bin;
-    gather<C>(s, base, n, [&](float x, int) {
-      const int b = bin_of(r, x);
-      return b >= 0 && b <= last && survives(s, r, x, b);
-    });
+    gather<T, C>(s, r, sl, base, 0, last, 0ull, ~0ull);
     if (rank == 0) {
       const int c = (int)s.n_list;             // exact survivors: at most `head`
       const u64 key = sorted(s, s.list, c);
@@ -710,14 +804,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     return;
   }
   if (cut_k) {
-    select<C>(s, r, base, n, true, (u64)k);
+    select<T, C>(r, sl, base, true, (u64)k);
     kept = s.res_mass;
   }
   if (cut_p) {
-    select<C>(s, r, base, n, false, reach(top_p, kept));
+    select<T, C>(r, sl, base, false, reach(top_p, kept));
     kept = s.res_mass;
   }
-  select<C>(s, r, base, n, false, reach(u, kept));
+  select<T, C>(r, sl, base, false, reach(u, kept));
   if (rank == 0 && t == 0) p.out[row] = s.res_idx;
 }
 

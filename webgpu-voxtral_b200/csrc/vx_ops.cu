@@ -270,8 +270,8 @@ cudaError_t launch_attention(pattn::Params p, const vx_kv_pages& c, const Plan& 
 template <typename T, int C>
 cudaError_t launch_sample(const sample::Params& p, int rows, cudaStream_t s) {
   static std::atomic<int> done[kMaxDevices];
-  const size_t bytes = sizeof(sample::Smem) + (size_t)p.slice * 4;
-  cudaError_t ce = allow_smem(sample::k_sample<T, C>, done, sizeof(sample::Smem) + sample::kMaxSlice * 4);
+  const size_t bytes = sizeof(sample::Smem) + (p.resident ? (size_t)p.slice * 4 : 0);
+  cudaError_t ce = allow_smem(sample::k_sample<T, C>, done, sizeof(sample::Smem) + sample::kResident * 4);
   if (ce != cudaSuccess) return ce;
   return launch_cluster(C, sample::k_sample<T, C>, dim3((unsigned)rows * C), dim3(sample::kThreads), bytes, s, p);
 }
@@ -375,7 +375,7 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   const Err e{err, err_len};
   if (!ap) return e.fail(VX_E_INVALID, "arguments are null");
   const vx_sample_args& a = *ap;
-  constexpr int most = sample::kMaxSlice * sample::kMaxCluster;
+  constexpr int most = sample::kMaxCols;
   if (a.dtype < 0 || a.dtype > 2) return e.fail(VX_E_INVALID, "dtype %d (0 F16, 1 BF16, 2 F32)", a.dtype);
   if (a.n_rows < 0 || a.n_cols < 1 || a.n_cols > most || a.row_stride < 0)
     return e.fail(VX_E_RANGE, "%d rows of %d logits (1 to %d), stride %lld", a.n_rows, a.n_cols, most, (long long)a.row_stride);
@@ -389,9 +389,11 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   if (reinterpret_cast<uintptr_t>(a.logits) % elem_size(a.dtype)) return e.fail(VX_E_INVALID, "logits must be aligned to their type");
   const int sms = sm_count();
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
-  // CTAs a row: slices of at most 16384 logits, so that two CTAs share an SM
+  // CTAs a row: more of them while all rows together give an SM less than one and a half (two fit),
+  // none with fewer than 8192 logits.  One B200: 64 rows of 131072 bf16 logits with 2, 4, 8 CTAs a row
+  // 47, 35, 43 us; 200 rows of f32 with 1, 2, 4 158, 143, 162 us; one row with 1, 4, 8 95, 36, 26 us
   int cluster = 1;
-  while (cluster < sample::kMaxCluster && (a.n_cols + cluster - 1) / cluster > 16384) cluster *= 2;
+  while (cluster < sample::kMaxCluster && 2ll * a.n_rows * cluster < 3ll * sms && a.n_cols > 8192 * cluster) cluster *= 2;
   if ((long long)a.n_rows * cluster > 0x7fffffff) return e.fail(VX_E_RANGE, "%d rows are too many for one call", a.n_rows);
   sample::Params p{};
   p.logits = a.logits; p.stride = a.row_stride; p.u = a.u;
@@ -399,6 +401,7 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   p.temperature1 = a.temperature_all; p.top_p1 = a.top_p_all; p.min_p1 = a.min_p_all; p.top_k1 = a.top_k_all;
   p.out = a.out; p.n = a.n_cols;
   p.slice = ((a.n_cols + cluster - 1) / cluster + 7) & ~7;
+  p.resident = p.slice <= sample::kResident;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t ce = a.dtype == 0 ? launch_sample<__half>(p, a.n_rows, cluster, s)
                          : a.dtype == 1 ? launch_sample<__nv_bfloat16>(p, a.n_rows, cluster, s) : launch_sample<float>(p, a.n_rows, cluster, s);
