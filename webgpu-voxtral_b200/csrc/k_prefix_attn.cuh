@@ -34,13 +34,20 @@ struct Params {
   const int32_t *prefix_pages, *page_table, *suffix_lens, *cu_q;   // cu_q null: one token each
   long long table_stride;
   int32_t* status;
-  float *part_o, *part_ml;   // [split][n_tokens * n_heads][D] / [..][2]
+  float* tile_o;             // partials of the tile kernel: [split][n_tokens * n_heads][D]
+  float2* tile_ml;
+  float* row_o;              // partials of the row kernel: [part][8 NT][D]
+  float2* row_ml;
+  int2* row_parts;           // [n_tokens * n_heads]: first and last partial row; last -1: none, -2: out is written
   int n_tokens, n_seqs, n_heads, n_kv, group;
   int prefix_len, page_size, n_pages, max_pages;
   float scale_log2;          // scale * log2(e): weights are 2^(s * scale_log2 - m)
-  int splits, split0;        // this launch's key ranges are partials [split0, split0 + splits)
-  int direct;                // one range in all: write out, no partials
-  int own_only;              // skip the prefix keys
+  int tile_parts;            // key ranges of the tile kernel (0: it does not run)
+  int row_rows;              // partial rows there is room for
+  int rows_run;              // whether the row kernel runs, and the rows of its tiles
+  int own_only;              // the row kernel leaves the prefix to the tile kernel
+  int min_blocks;            // blocks a warp of the row kernel takes at least
+  int direct;                // the tile kernel alone, with one key range: it writes out
 };
 
 template <typename T>
@@ -93,152 +100,300 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // ---------------------------------------------------------------- short row tiles
-// A CTA takes up to 8 NT query rows of one sequence that share a K/V head (row = query token
-// x group + head of the group) and one range of their keys.  Its 4 warps take 16-key blocks
-// in turn, each through a ring of its own (cp.async, no block-wide barrier in the loop).
+// Up to 8 NT query rows of one sequence that share a K/V head are an item; its work is the 16-key
+// blocks of its sequence.  All blocks of all items stand in one line (sequence, row tile, head, block)
+// that the warps of the grid share out evenly, whatever the lengths are: a warp takes `per` blocks in a
+// row, through a ring of its own (cp.async, no block-wide barrier in the loop), and leaves one partial
+// for each item that it meets.  Warp w's part of item i is partial w + i: no two parts share a
+// number, since from one part to the next w or i goes up, and the parts of an item follow one another.
 // Scores are formed transposed, S^T = K Q^T (16 keys x 8 rows an MMA), so that 4 query heads
 // fill half of an MMA's rows and not a quarter; P^T comes from S^T by an 8x8 register transpose
 // and O^T = V^T P^T.
-constexpr int kRowWarps = 4;
+//
+// Bound: the reading of K and V (HBM, or L2 where sequences read the same prefix).
 constexpr int kRowStages = 3;
-template <int D>
+// Warps of a CTA, one CTA an SM: as many as shared memory holds rings for (registers allow them too).
+constexpr int row_warps(int d, int nt) {
+  return d == 128 ? (nt == 1 ? 7 : nt == 2 ? 6 : 4) : (nt == 1 ? 14 : nt == 2 ? 12 : 8);
+}
+template <int D, int NT>
+constexpr int row_warp_smem() {   // K and V of the stages, the query rows of as many items, what each stage holds
+  return kRowStages * (2 * 16 * D * 2 + 8 * NT * D * 2 + 64);
+}
+template <int D, int NT>
 constexpr int row_smem() {
-  return kRowWarps * kRowStages * 2 * 16 * D * 2;
+  return row_warps(D, NT) * row_warp_smem<D, NT>();
 }
 
-// Tile `z` of the grid: its sequence and the tile's number in it (warp-wide, all lanes).
-__device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int lane, int& b, int& i) {
-  if (!p.cu_q) {
-    const int per = (p.group + rows - 1) / rows;
-    b = z / per;
-    i = z - b * per;
-    return b < p.n_seqs;
+// A sequence as the row kernel sees it.
+struct Seq {
+  int tok0, nq, own, tiles, blocks;   // query tokens, own keys, row tiles, 16-key blocks (prefix and own)
+  __device__ __forceinline__ long long units(int n_kv) const { return (long long)tiles * n_kv * blocks; }
+};
+__device__ __forceinline__ Seq sequence(const Params& p, int b, int rows) {
+  Seq q{0, 0, 0, 0, 0};
+  if (b >= p.n_seqs) return q;
+  q.tok0 = p.cu_q ? p.cu_q[b] : b;
+  q.nq = p.cu_q ? p.cu_q[b + 1] - q.tok0 : 1;
+  const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
+  q.own = max(0, min(given, cap));
+  if (given > cap) ops::report(p.status, kDevBadIndex);       // keys that the page table does not hold
+  if (q.tok0 < 0 || q.nq < 0 || q.tok0 + q.nq > p.n_tokens) {   // offsets that the batch does not hold
+    ops::report(p.status, kDevBadIndex);
+    q.nq = 0;
   }
-  int before = 0;
-  for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
-    int n = 0;
-    if (b0 + lane < p.n_seqs) n = (max(0, p.cu_q[b0 + lane + 1] - p.cu_q[b0 + lane]) * p.group + rows - 1) / rows;
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > z);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      b = b0 + l;
-      i = z - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, n, l));
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return false;
+  q.tiles = (q.nq * p.group + rows - 1) / rows;
+  q.blocks = (p.own_only ? 0 : (p.prefix_len + 15) / 16) + (q.own + 15) / 16;
+  return q;
 }
+
+// What a stage of the ring holds.
+struct Stage {
+  int keys, pos;            // keys of the block that exist, position of its first
+  int flags;                // 1: first block of the warp's part, 2: its last, 4: the item's first, 8: the item's last
+  int tok0, first_lim;      // the sequence's first query token, and the keys that it sees
+  int row0, n_rows, kvh;    // the item
+  int item, q_slot;
+};
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kRowWarps * 32) k_attn_rows(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __grid_constant__ Params p) {
   using E = ops::Elem<T>;
-  constexpr int ROWS = 8 * NT, KK = D / 16, CH = D / 8, TILE = 16 * D * 2;
+  constexpr int ROWS = 8 * NT, KK = D / 16, CH = D / 8, TILE = 16 * D * 2, kRowWarps = row_warps(D, NT), RUN = kRowWarps * 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[kRowWarps][ROWS], s_l[kRowWarps][ROWS];
+  __shared__ long long s_sum[kRowWarps], s_start;
+  __shared__ int s_items[kRowWarps], s_start_items, s_start_seq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = blockIdx.z, kvh = blockIdx.y;
   griddep_launch();
   griddep_wait();
-  int b, ti;
-  if (!find_tile(p, blockIdx.x, ROWS, lane, b, ti)) return;
-  const int tok0 = p.cu_q ? p.cu_q[b] : b;
-  const int nq = p.cu_q ? p.cu_q[b + 1] - tok0 : 1;
-  const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
-  const int own = max(0, min(given, cap));
-  if (given > cap && threadIdx.x == 0) ops::report(p.status, kDevBadIndex);   // keys that the page table does not hold
-  const int n_rows = min(ROWS, nq * p.group - ti * ROWS);
-  if (tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) {   // offsets that the batch does not hold
-    if (threadIdx.x == 0) ops::report(p.status, kDevBadIndex);
-    return;
-  }
-  const int first_lim = p.prefix_len + own - nq + 1;   // keys that query token 0 sees
-  // 16-key blocks of this tile: the prefix's, then the sequence's own
-  const int last_lim = max(0, first_lim + (ti * ROWS + n_rows - 1) / p.group);
-  const int pre_blocks = (min(p.prefix_len, last_lim) + 15) / 16;
-  const int blk0 = p.own_only ? pre_blocks : 0;
-  const int n_blocks = pre_blocks + (max(0, last_lim - p.prefix_len) + 15) / 16 - blk0;
-  const int per = max(((n_blocks + p.splits - 1) / p.splits + kRowWarps - 1) / kRowWarps * kRowWarps, 4 * kRowWarps);
-  const int begin = blk0 + split * per, end = min(blk0 + n_blocks, begin + per);
 
-  // query fragments (B operand): lane holds row lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each 16
-  uint32_t qf[NT][KK][2];
-  int lim[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = ti * ROWS + n * 8 + (lane >> 2);
-    const bool live = n * 8 + (lane >> 2) < n_rows;
-    const int j = r / p.group, g = r - j * p.group;
-    const T* src = (const T*)p.q + (long long)(tok0 + j) * p.q_tok + (long long)(kvh * p.group + g) * p.q_head + 2 * (lane & 3);
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      qf[n][k][0] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-      qf[n][k][1] = live ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int c = n * 8 + 2 * (lane & 3) + e;
-      lim[n][e] = c < n_rows ? first_lim + (ti * ROWS + c) / p.group : 0;
-    }
+  // ---- the line: its length, and the run of sequences in which this CTA's part begins
+  const int n_chunks = (p.n_seqs + RUN - 1) / RUN;
+  long long total = 0;
+  for (int c = 0; c < n_chunks; ++c) {
+    const int b = c * RUN + threadIdx.x;
+    const Seq q = sequence(p, b, ROWS);
+    if (q.tiles && !q.blocks && b % (int)gridDim.x == (int)blockIdx.x)   // no keys: no part of any warp
+      for (long long r = (long long)q.tok0 * p.n_heads; r < (long long)(q.tok0 + q.nq) * p.n_heads; ++r) p.row_parts[r] = make_int2(0, -1);
+    long long u = q.units(p.n_kv);
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if (lane == 0) s_sum[warp] = u;
+    __syncthreads();
+    for (int w = 0; w < kRowWarps; ++w) total += s_sum[w];
+    __syncthreads();
   }
-
-  const uint32_t ring = smem_u32(smem) + warp * (kRowStages * 2 * TILE);
-  const T* kb = (const T*)p.k.base + kvh * p.k.head;
-  const T* vb = (const T*)p.v.base + kvh * p.v.head;
-  auto issue = [&](int blk, int st) {
-    if (blk < end) {
-      const bool pre = blk < pre_blocks;
-      const int key = 16 * (pre ? blk : blk - pre_blocks);
-      const int n = (pre ? p.prefix_len : own) - key;   // keys of the block that exist
-      const int lp = key / p.page_size;
-      int page = -1;
-      if (pre) page = p.prefix_pages[lp];
-      else if (lp < p.max_pages) page = p.page_table[(long long)b * p.table_stride + lp];
-      const bool ok = page >= 0 && page < p.n_pages;
-      if (!ok) {
-        ops::report(p.status, kDevBadIndex);
-        page = 0;
+  const long long warps = (long long)gridDim.x * kRowWarps;
+  const long long per = max((total + warps - 1) / warps, (long long)p.min_blocks);
+  const long long cta_first = (long long)blockIdx.x * kRowWarps * per;
+  if (cta_first >= total) return;
+  if (n_chunks > 1) {
+    long long before = 0;
+    int items = 0;
+    for (int c = 0; c < n_chunks; ++c) {
+      const Seq q = sequence(p, c * RUN + threadIdx.x, ROWS);
+      long long u = q.units(p.n_kv);
+      int it = q.tiles * p.n_kv;
+      for (int o = 16; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        it += __shfl_xor_sync(0xffffffffu, it, o);
       }
-      const int slot = key % p.page_size;
-      const T* ks = kb + page * p.k.page + slot * p.k.slot;
-      const T* vs = vb + page * p.v.page + slot * p.v.slot;
-      const uint32_t dst = ring + st * 2 * TILE;
+      if (lane == 0) {
+        s_sum[warp] = u;
+        s_items[warp] = it;
+      }
+      __syncthreads();
+      long long sum = 0;
+      int its = 0;
+      for (int w = 0; w < kRowWarps; ++w) {
+        sum += s_sum[w];
+        its += s_items[w];
+      }
+      if (before + sum > cta_first || c == n_chunks - 1) {   // the same in every thread
+        if (threadIdx.x == 0) {
+          s_start = before;
+          s_start_items = items;
+          s_start_seq = c * RUN;
+        }
+        break;
+      }
+      before += sum;
+      items += its;
+      __syncthreads();
+    }
+  } else if (threadIdx.x == 0) {
+    s_start = 0;
+    s_start_items = s_start_seq = 0;
+  }
+  __syncthreads();
+
+  const long long w_id = (long long)blockIdx.x * kRowWarps + warp;
+  const long long u0 = w_id * per;
+  long long u1 = min(total, u0 + per);
+  if (u0 >= total) return;                     // whole warps; no barrier follows
+
+  // ---- the issuing side: where the warp stands in the line
+  long long before = s_start;                  // units and items before sequence `chunk`
+  int items = s_start_items, chunk = s_start_seq;
+  Seq q{};
+  int b = 0, in_item = 0, blk = 0, part_left = 0, q_count = 0, page_lane = 0, page_from = 0;
+  bool part_starts = false;
+  long long u = u0;
+  uint8_t* mine = smem + warp * row_warp_smem<D, NT>();
+  const uint32_t ring = smem_u32(mine), q_ring = ring + kRowStages * 2 * TILE;
+  Stage* stages = reinterpret_cast<Stage*>(mine + kRowStages * (2 * TILE + ROWS * D * 2));
+  int item_base = 0;                           // number of the sequence's first item
+
+  // the sequence that holds unit u, all lanes together
+  const auto locate = [&]() {
+    while (true) {
+      const Seq x = sequence(p, chunk + lane, ROWS);
+      const long long n = x.units(p.n_kv);
+      long long incl = n;
+      int it = x.tiles * p.n_kv, it_incl = it;
 #pragma unroll
-      for (int c = 0; c < 16 * CH / 32; ++c) {
-        const int x = c * 32 + lane, row = x / CH, col = x % CH;
-        const uint32_t at = dst + row * (D * 2) + ((col ^ (row & 7)) << 4);
-        const bool live = ok && row < n;
-        cp16(at, live ? ks + row * p.k.slot + col * 8 : ks, live);
-        cp16(at + TILE, live ? vs + row * p.v.slot + col * 8 : vs, live);
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+        const int z = __shfl_up_sync(0xffffffffu, it_incl, o);
+        if (lane >= o) {
+          incl += y;
+          it_incl += z;
+        }
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + incl > u);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = chunk + l;
+        q.tok0 = __shfl_sync(0xffffffffu, x.tok0, l);
+        q.nq = __shfl_sync(0xffffffffu, x.nq, l);
+        q.own = __shfl_sync(0xffffffffu, x.own, l);
+        q.tiles = __shfl_sync(0xffffffffu, x.tiles, l);
+        q.blocks = __shfl_sync(0xffffffffu, x.blocks, l);
+        item_base = items + __shfl_sync(0xffffffffu, it_incl - it, l);
+        const long long off = u - (before + __shfl_sync(0xffffffffu, incl - n, l));
+        in_item = (int)(off / q.blocks);
+        blk = (int)(off - (long long)in_item * q.blocks);
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      items += __shfl_sync(0xffffffffu, it_incl, 31);
+      chunk += 32;
+      if (chunk >= p.n_seqs) {                 // not reached while the lengths stay what they were
+        u1 = u;
+        return;
+      }
+    }
+  };
+  const int pre_blocks = p.own_only ? 0 : (p.prefix_len + 15) / 16;
+  const auto issue = [&](int st) {
+    if (u < u1) {
+      if (part_left == 0) {                    // the next part: the rest of this item, or of this warp's units
+        if (u == u0 || in_item + 1 >= q.tiles * p.n_kv) {
+          locate();
+        } else {
+          ++in_item;
+          blk = 0;
+        }
+        part_left = (int)min((long long)(q.blocks - blk), u1 - u);
+        part_starts = true;
+        page_from = -64;
+      }
+      if (u < u1) {
+        const int ti = in_item / p.n_kv, kvh = in_item - ti * p.n_kv;
+        const bool pre = blk < pre_blocks;
+        const int key = 16 * (pre ? blk : blk - pre_blocks);
+        const int keys = (pre ? p.prefix_len : q.own) - key;
+        // page numbers of 32 blocks at once, a block a lane
+        if (blk - page_from >= 32) {
+          page_from = blk;
+          const int bl = blk + lane;
+          const bool bp = bl < pre_blocks;
+          const int lp = 16 * (bp ? bl : bl - pre_blocks) / p.page_size;
+          page_lane = -1;
+          if (bl < blk + part_left) {
+            if (bp) page_lane = p.prefix_pages[lp];
+            else if (lp < p.max_pages) page_lane = p.page_table[(long long)b * p.table_stride + lp];
+            if (page_lane < 0 || page_lane >= p.n_pages) {
+              ops::report(p.status, kDevBadIndex);
+              page_lane = -1;
+            }
+          }
+        }
+        const int page = __shfl_sync(0xffffffffu, page_lane, blk - page_from);
+        const bool ok = page >= 0;
+        const int slot = key % p.page_size;
+        const T* ks = (const T*)p.k.base + kvh * p.k.head + (ok ? page : 0) * p.k.page + slot * p.k.slot;
+        const T* vs = (const T*)p.v.base + kvh * p.v.head + (ok ? page : 0) * p.v.page + slot * p.v.slot;
+        const uint32_t dst = ring + st * 2 * TILE;
+#pragma unroll
+        for (int c = 0; c < 16 * CH / 32; ++c) {
+          const int x = c * 32 + lane, row = x / CH, col = x % CH;
+          const uint32_t at = dst + row * (D * 2) + ((col ^ (row & 7)) << 4);
+          const bool live = ok && row < keys;
+          cp16(at, live ? ks + row * p.k.slot + col * 8 : ks, live);
+          cp16(at + TILE, live ? vs + row * p.v.slot + col * 8 : vs, live);
+        }
+        const int row0 = ti * ROWS, n_rows = min(ROWS, q.nq * p.group - row0);
+        if (part_starts) {
+          ++q_count;
+#pragma unroll 1
+          for (int x = lane; x < ROWS * CH; x += 32) {
+            const int row = x / CH, col = x % CH;
+            const bool live = row < n_rows;
+            const int j = (row0 + row) / p.group, g = row0 + row - j * p.group;
+            const T* src = (const T*)p.q + (live ? (long long)(q.tok0 + j) * p.q_tok + (long long)(kvh * p.group + g) * p.q_head + col * 8 : 0);
+            cp16(q_ring + (q_count % kRowStages) * ROWS * D * 2 + row * (D * 2) + ((col ^ (row & 7)) << 4), src, live);
+          }
+        }
+        if (lane == 0)
+          stages[st] = Stage{keys, (pre ? 0 : p.prefix_len) + key,
+                             (part_starts ? 1 : 0) | (part_left == 1 ? 2 : 0) | (blk == 0 ? 4 : 0) | (blk == q.blocks - 1 ? 8 : 0), q.tok0,
+                             p.prefix_len + q.own - q.nq + 1, row0, n_rows, kvh, item_base + in_item, q_count % kRowStages};
+        part_starts = false;
+        ++blk;
+        --part_left;
+        ++u;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
+  uint32_t qf[NT][KK][2];
+  int lim[NT][2];
   float m[NT][2], l[NT][2], o[NT][KK][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int d = 0; d < KK; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
-  }
-#pragma unroll
-  for (int s = 0; s < kRowStages - 1; ++s) issue(begin + warp + s * kRowWarps, s);
+  for (int s = 0; s < kRowStages - 1; ++s) issue(s);
   int st = 0;
-  for (int blk = begin + warp; blk < end; blk += kRowWarps) {
+  bool item_first = false;                     // the warp's part holds the item's first block
+  for (long long i = u0; i < u1; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
     __syncwarp();
-    issue(blk + (kRowStages - 1) * kRowWarps, st == 0 ? kRowStages - 1 : st - 1);
+    const Stage sg = stages[st];
     const uint32_t kt = ring + st * 2 * TILE, vt = kt + TILE;
-    st = st + 1 == kRowStages ? 0 : st + 1;
     const int mat = lane >> 3, r8 = lane & 7;
+    if (sg.flags & 1) {
+      item_first = sg.flags & 4;
+      // query fragments (B operand): lane holds row lane / 4, values 2 (lane % 4) + {0, 1, 8, 9} of each 16
+      const uint32_t qs = q_ring + sg.q_slot * ROWS * D * 2;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int k = 0; k < KK; k += 2) {
+          const int row = n * 8 + r8, col = 2 * k + mat;
+          ldmatrix_x4(qf[n][k][0], qf[n][k][1], qf[n][k + 1][0], qf[n][k + 1][1], qs + row * (D * 2) + ((col ^ (row & 7)) << 4));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = n * 8 + 2 * (lane & 3) + e;
+          lim[n][e] = c < sg.n_rows ? sg.first_lim + (sg.row0 + c) / p.group : 0;
+          m[n][e] = -INFINITY;
+          l[n][e] = 0.f;
+        }
+#pragma unroll
+        for (int d = 0; d < KK; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
+      }
+    }
+    issue(st == 0 ? kRowStages - 1 : st - 1);
+    st = st + 1 == kRowStages ? 0 : st + 1;
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -251,10 +406,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_attn_rows(const __grid_const
       for (int n = 0; n < NT; ++n) mma16816<T>(s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
     }
     // lane holds keys lane / 4 and + 8, rows 2 (lane % 4) and + 1 of each tile of 8
-    const bool pre = blk < pre_blocks;
-    const int key = 16 * (pre ? blk : blk - pre_blocks) + (lane >> 2);
-    const int left = (pre ? p.prefix_len : own) - key;      // > 0: the key exists
-    const int pos = (pre ? 0 : p.prefix_len) + key;
+    const int left = sg.keys - (lane >> 2);      // > 0: the key exists
+    const int pos = sg.pos + (lane >> 2);
     uint32_t pb[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -295,60 +448,77 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_attn_rows(const __grid_const
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma16816<T>(o[n][d], a0, a1, a2, a3, pb[n][0], pb[n][1]);
     }
+    if (sg.flags & 2) {
+      // the part is done: the rows' sums, and the result or a partial
+      const bool whole = item_first && (sg.flags & 8) && !p.tile_parts;
+      const long long part = w_id + sg.item;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+          l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+          l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+          const int c = n * 8 + 2 * (lane & 3) + e;
+          if (c < sg.n_rows) {
+            const int j = (sg.row0 + c) / p.group, g = sg.row0 + c - j * p.group;
+            const long long tok = sg.tok0 + j;
+            const int head = sg.kvh * p.group + g;
+            const long long row = tok * p.n_heads + head;
+            if (whole) {
+              const float inv = l[n][e] > 0.f ? 1.f / l[n][e] : 0.f;
+              T* dst = (T*)p.out + tok * p.o_tok + head * p.o_head + (lane >> 2);
+#pragma unroll
+              for (int d = 0; d < KK; ++d) {
+                dst[d * 16] = E::from_f32(o[n][d][e] * inv);
+                dst[d * 16 + 8] = E::from_f32(o[n][d][e + 2] * inv);
+              }
+              if (lane < 4) p.row_parts[row] = make_int2(0, -2);
+            } else {
+              float* dst = p.row_o + (part * ROWS + c) * D + (lane >> 2);
+              if (m[n][e] != -INFINITY)
+#pragma unroll
+                for (int d = 0; d < KK; ++d) {
+                  dst[d * 16] = o[n][d][e];
+                  dst[d * 16 + 8] = o[n][d][e + 2];
+                }
+              if (lane < 4) {
+                p.row_ml[part * ROWS + c] = make_float2(m[n][e], l[n][e]);
+                // where the row's partials begin and end, ROWS apart
+                if (item_first) p.row_parts[row].x = (int)(part * ROWS + c);
+                if (sg.flags & 8) p.row_parts[row].y = (int)(part * ROWS + c);
+              }
+            }
+          }
+        }
+    }
     __syncwarp();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
 
-  // ---- the 4 warps' states join in shared memory
+// Tile `z` of a ragged grid: its sequence and the tile's number in it (warp-wide, all lanes).
+__device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int lane, int& b, int& i) {
+  int before = 0;
+  for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+    int n = 0;
+    if (b0 + lane < p.n_seqs) n = (max(0, p.cu_q[b0 + lane + 1] - p.cu_q[b0 + lane]) * p.group + rows - 1) / rows;
+    int incl = n;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
-      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
-      l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
-      if (lane < 4) {
-        s_m[warp][n * 8 + 2 * lane + e] = m[n][e];
-        s_l[warp][n * 8 + 2 * lane + e] = l[n][e];
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
     }
-  __syncthreads();   // the rings are free
-  float* so = reinterpret_cast<float*>(smem);   // [warp][ROWS][D]
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int d = 0; d < KK; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        so[(warp * ROWS + n * 8 + 2 * (lane & 3) + (e & 1)) * D + d * 16 + (lane >> 2) + (e >> 1) * 8] = o[n][d][e];
-  __syncthreads();
-  for (int x = threadIdx.x; x < n_rows * (D / 4); x += kRowWarps * 32) {
-    const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
-    float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, s_m[w][r]);
-    const float m_use = M == -INFINITY ? 0.f : M;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-      const float f = ex2(s_m[w][r] - m_use);
-      const float4 v = *reinterpret_cast<const float4*>(so + (w * ROWS + r) * D + d);
-      L += s_l[w][r] * f;
-      acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > z);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      b = b0 + l;
+      i = z - before - (__shfl_sync(0xffffffffu, incl, l) - __shfl_sync(0xffffffffu, n, l));
+      return true;
     }
-    const int lr = ti * ROWS + r, j = lr / p.group, g = lr - j * p.group;
-    const long long tok = tok0 + j;
-    const int head = kvh * p.group + g;
-    if (p.direct) {
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      *reinterpret_cast<uint2*>((T*)p.out + tok * p.o_tok + head * p.o_head + d) =
-          make_uint2(E::pack(acc.x * inv, acc.y * inv), E::pack(acc.z * inv, acc.w * inv));
-    } else {
-      const long long row = (long long)(p.split0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
-      if (M != -INFINITY) *reinterpret_cast<float4*>(p.part_o + row * D + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * row) = make_float2(M, L);
-    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
+  return false;
 }
 
 // ---------------------------------------------------------------- tiles of 128 rows
@@ -455,7 +625,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   const int row0 = ti * 2 * kTile;                       // first row: token tok0 + row / group, head row % group
   const int n_pre = (min(p.prefix_len, last_lim) + kTile - 1) / kTile;
   const int n_all = n_pre + (max(0, last_lim - p.prefix_len) + kTile - 1) / kTile;
-  const int per = (n_all + p.splits - 1) / p.splits;
+  const int per = (n_all + p.tile_parts - 1) / p.tile_parts;
   const int t0 = split * per, n = max(0, min(n_all, t0 + per) - t0);
   const int n_tiles = n_rows > kTile ? 2 : 1;
 
@@ -674,9 +844,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         const bool live = lr < n_rows;
         const long long tok = tok0 + (row0 + lr) / p.group;
         const int head = kvh * p.group + (row0 + lr) % p.group;
-        const long long at = (long long)(p.split0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
+        const long long at = (long long)split * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        if (live && !p.direct) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, l);
+        if (live && !p.direct) p.tile_ml[at] = make_float2(m, l);
         // rows to memory by one bulk copy each, staged in the ring (free now); 16 bytes of padding
         // keep the threads' rows on different banks
         const int row_bytes = p.direct ? D * 2 : D * 4;
@@ -703,7 +873,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         }
         fence_async_smem();
         if (live && (p.direct || m != -INFINITY)) {
-          void* dst = p.direct ? (void*)((T*)p.out + tok * p.o_tok + (long long)head * p.o_head) : (void*)(p.part_o + at * D);
+          void* dst = p.direct ? (void*)((T*)p.out + tok * p.o_tok + (long long)head * p.o_head) : (void*)(p.tile_o + at * D);
           bulk_s2g(dst, smem_u32(stage), row_bytes);
         }
       }
@@ -719,51 +889,75 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
 }
 
 // ---------------------------------------------------------------- joining key ranges
-// One warp per row (token, head): weights of the ranges from their (m, l), then the weighted
-// sum of their o.  Ranges are added in order, so the result does not depend on timing.
+// One warp per row (token, head): the maximum over its partials, then the weighted sums in the
+// order of the partials, so the result does not depend on timing.  Four weights and four partials are on their
+// way at a time.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Params p) {
   using E = ops::Elem<T>;
   constexpr int V = D / 32;   // values a lane
   griddep_launch();
   griddep_wait();
   const long long rows = (long long)p.n_tokens * p.n_heads;
-  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
+  const long long tok = row / p.n_heads;
+  if (p.cu_q && (tok < p.cu_q[0] || tok >= p.cu_q[p.n_seqs])) return;   // no sequence's token
+  int2 parts = make_int2(0, -1);
+  if (p.rows_run) parts = __ldcg(p.row_parts + row);
+  if (parts.y == -2) return;
+  if (parts.x < 0 || parts.y < parts.x || parts.y >= p.row_rows) parts = make_int2(0, -1);   // offsets that the row kernel refused
+  const int n_row = parts.y < 0 ? 0 : (parts.y - parts.x) / p.rows_run + 1, n = p.tile_parts + n_row;
+  // partial s: the tile kernel's key ranges first
+  const auto ml_of = [&](int s) {
+    return s < p.tile_parts ? __ldcg(p.tile_ml + s * rows + row) : __ldcg(p.row_ml + parts.x + (long long)(s - p.tile_parts) * p.rows_run);
+  };
+  const auto o_of = [&](int s) {
+    return (s < p.tile_parts ? p.tile_o + (s * rows + row) * D : p.row_o + (parts.x + (long long)(s - p.tile_parts) * p.rows_run) * D) + lane * V;
+  };
   float M = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) M = fmaxf(M, __ldcg(p.part_ml + 2 * (s * rows + row)));
+  for (int s = lane; s < n; s += 32) M = fmaxf(M, ml_of(s).x);
   M = warp_max(M);
   const float m_use = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 32) {
+  for (int s0 = 0; s0 < n; s0 += 32) {
     float f = 0.f;
-    if (s0 + lane < p.splits) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * ((s0 + lane) * rows + row)));
+    if (s0 + lane < n) {
+      const float2 ml = ml_of(s0 + lane);
       f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m_use);
       L += ml.y * f;
     }
-    const int n = min(32, p.splits - s0);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float w = __shfl_sync(0xffffffffu, f, s);
-      if (w == 0.f) continue;   // a range without keys left its o unwritten
-      const float* o = p.part_o + ((s0 + s) * rows + row) * D + lane * V;
-      if constexpr (V == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
-        acc[0] += v.x * w; acc[1] += v.y * w; acc[2] += v.z * w; acc[3] += v.w * w;
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(o));
-        acc[0] += v.x * w; acc[1] += v.y * w;
+    const int k = min(32, n - s0);
+    for (int s = 0; s < k; s += 4) {
+      float w[4], v[4][V];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = __shfl_sync(0xffffffffu, f, (s + j) & 31);
+        if (s + j >= k) w[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = 0.f;
+        if (w[j] != 0.f) {   // a range without keys left its o unwritten
+          const float* o = o_of(s0 + s + j);
+          if constexpr (V == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(o));
+            v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
+          } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(o));
+            v[j][0] = x.x; v[j][1] = x.y;
+          }
+        }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += v[j][i] * w[j];
     }
   }
   L = warp_sum(L);
   const float inv = L > 0.f ? 1.f / L : 0.f;
-  const long long tok = row / p.n_heads;
-  if (p.cu_q && (tok < p.cu_q[0] || tok >= p.cu_q[p.n_seqs])) return;   // no sequence's token
   const int head = (int)(row - tok * p.n_heads);
   T* dst = (T*)p.out + tok * p.o_tok + head * p.o_head + lane * V;
   if constexpr (V == 4) {

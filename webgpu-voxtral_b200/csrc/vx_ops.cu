@@ -35,6 +35,7 @@ struct Err {
 };
 
 constexpr int kMaxDevices = 64;
+constexpr double kSharePrefixBytes = 50e6;
 
 int sm_count() {
   static std::atomic<int> known[kMaxDevices];
@@ -119,18 +120,18 @@ cudaError_t launch_append(const append::Params& p, int interleaved, cudaStream_t
 
 // ------------------------------------------------------------------ attention
 struct Plan {
-  int nt;               // row kernel: tiles of 8 nt rows; 0: not launched
-  long long row_tiles;
-  int row_splits;
   int own;              // tile kernel over prefix and own keys (1) or the shared prefix alone (0)
   long long pairs;      // tile kernel: pairs of 128-row tiles; 0: not launched
-  int tile_splits;
+  int tile_parts;
+  int nt;               // row kernel: tiles of 8 nt rows; 0: not launched
+  int row_ctas;
+  int64_t tile_rows, row_rows;   // partial rows of each kernel
   int64_t bytes;
 };
 
 // Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's
 // share of the key tiles least, a range's start and end counted as two tiles.
-int tile_splits(long long items, long long tiles, int sms) {
+int tile_parts(long long items, long long tiles, int sms) {
   int best = 1;
   double least = 1e300;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {
@@ -169,30 +170,30 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   const long long own_keys = (long long)a.max_pages * c.page_size, rows = (long long)a.n_tokens * group;
   pl = Plan{};
   // The tile kernel multiplies 128 rows at once; below 64 rows a sequence the row kernel's tiles
-  // of 32 waste less.  One token a sequence: the prefix goes to the tile kernel, all sequences together.
+  // of 32 waste less.
   pl.own = a.cu_q && rows >= 64ll * a.n_seqs;
   if (pl.own) {
     pl.pairs = rows / 256 + a.n_seqs;
-    pl.tile_splits = tile_splits(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128 + (own_keys + 127) / 128, sms);
+    pl.tile_parts = tile_parts(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128 + (own_keys + 127) / 128, sms);
   } else {
-    if (!a.cu_q && a.n_seqs > 1 && a.prefix_len >= 128) {
+    // One token a sequence: all sequences' rows take the prefix together in the tile kernel, where
+    // reading it for each of them (from L2, 8 MB a us) would take longer than that kernel's start and end
+    if (!a.cu_q && (double)a.n_seqs * a.prefix_len * c.n_kv_heads * c.head_dim * 4 > kSharePrefixBytes) {
       pl.pairs = (rows + 255) / 256;
-      pl.tile_splits = tile_splits(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
+      pl.tile_parts = tile_parts(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
     }
-    const long long keys = own_keys + (pl.pairs ? 0 : a.prefix_len);
-    if (keys || !pl.pairs) {
+    if (own_keys || !pl.pairs) {
       pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
-      const int tile = 8 * pl.nt;
-      pl.row_tiles = a.cu_q ? rows / tile + a.n_seqs : (long long)a.n_seqs * ((group + tile - 1) / tile);
-      // enough CTAs for two waves of two an SM, 256 keys a range at least
-      const long long items = std::max(1ll, pl.row_tiles * c.n_kv_heads);
-      pl.row_splits = (int)std::max(1ll, std::min({(4ll * sms + items - 1) / items, (keys + 255) / 256, 64ll}));
+      pl.row_ctas = sms;
     }
   }
-  if (std::max(pl.pairs, pl.row_tiles) > 0x7fffffff)
+  const long long tile = 8 * pl.nt;
+  const long long items = !pl.nt ? 0 : (a.cu_q ? rows / tile + a.n_seqs : a.n_seqs * ((group + tile - 1) / tile)) * c.n_kv_heads;
+  pl.tile_rows = pl.pairs && (pl.nt || pl.tile_parts > 1) ? (int64_t)pl.tile_parts * a.n_tokens * a.n_heads : 0;
+  pl.row_rows = pl.nt ? ((int64_t)pl.row_ctas * pattn::row_warps(c.head_dim, pl.nt) + items) * tile : 0;
+  if (pl.pairs > 0x7fffffff || pl.row_rows > 0x7fffffff || (long long)a.n_tokens * a.n_heads > 0x7fffffff)
     return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
-  const int splits = pl.tile_splits + pl.row_splits;
-  pl.bytes = splits == 1 ? 0 : (int64_t)splits * a.n_tokens * a.n_heads * (c.head_dim + 2) * 4;
+  pl.bytes = (pl.tile_rows + pl.row_rows) * (c.head_dim + 2) * 4 + (pl.nt ? (int64_t)a.n_tokens * a.n_heads * 8 : 0);
   return VX_OK;
 }
 
@@ -224,13 +225,12 @@ cudaError_t encode_pages(CUtensorMap* map, const vx_kv_pages& c, const pattn::Pa
 }
 
 template <typename T, int D, int NT>
-cudaError_t launch_rows(const pattn::Params& p, long long tiles, cudaStream_t s) {
+cudaError_t launch_rows(const pattn::Params& p, int ctas, cudaStream_t s) {
   static std::atomic<int> done[kMaxDevices];
-  // the rings, and the warps' f32 states that take their place at the end
-  constexpr int bytes = std::max(pattn::row_smem<D>(), pattn::kRowWarps * 8 * NT * D * 4);
+  constexpr int bytes = pattn::row_smem<D, NT>();
   cudaError_t ce = allow_smem(pattn::k_attn_rows<T, D, NT>, done, bytes);
   if (ce != cudaSuccess) return ce;
-  return launch(pattn::k_attn_rows<T, D, NT>, dim3((unsigned)tiles, p.n_kv, p.splits), dim3(pattn::kRowWarps * 32), bytes, s, p);
+  return launch(pattn::k_attn_rows<T, D, NT>, dim3(ctas), dim3(pattn::row_warps(D, NT) * 32), bytes, s, p);
 }
 template <typename T, int D, bool OWN>
 cudaError_t launch_tiles(const pattn::Params& p, const vx_kv_pages& c, long long pairs, cudaStream_t s) {
@@ -241,29 +241,19 @@ cudaError_t launch_tiles(const pattn::Params& p, const vx_kv_pages& c, long long
   if (ce == cudaSuccess) ce = encode_pages(&km, c, p.k);
   if (ce == cudaSuccess) ce = encode_pages(&vm, c, p.v);
   if (ce != cudaSuccess) return ce;
-  return launch(pattn::k_attn_tiles<T, D, OWN>, dim3((unsigned)pairs, p.n_kv, p.splits), dim3(pattn::kTileThreads), bytes, s, km, vm, p);
+  return launch(pattn::k_attn_tiles<T, D, OWN>, dim3((unsigned)pairs, p.n_kv, p.tile_parts), dim3(pattn::kTileThreads), bytes, s, km, vm, p);
 }
 
 template <typename T, int D>
-cudaError_t launch_attention(pattn::Params p, const vx_kv_pages& c, const Plan& pl, cudaStream_t s) {
-  const int all = pl.tile_splits + pl.row_splits;
-  p.direct = all == 1;
+cudaError_t launch_attention(const pattn::Params& p, const vx_kv_pages& c, const Plan& pl, cudaStream_t s) {
   cudaError_t ce = cudaSuccess;
-  if (pl.pairs) {
-    p.splits = pl.tile_splits;
-    ce = pl.own ? launch_tiles<T, D, true>(p, c, pl.pairs, s) : launch_tiles<T, D, false>(p, c, pl.pairs, s);
-    p.split0 = pl.tile_splits;
-    p.own_only = 1;
-  }
-  if (ce == cudaSuccess && pl.row_tiles) {
-    p.splits = pl.row_splits;
-    ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.row_tiles, s)
-         : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.row_tiles, s) : launch_rows<T, D, 4>(p, pl.row_tiles, s);
-  }
+  if (pl.pairs) ce = pl.own ? launch_tiles<T, D, true>(p, c, pl.pairs, s) : launch_tiles<T, D, false>(p, c, pl.pairs, s);
+  if (ce == cudaSuccess && pl.nt)
+    ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.row_ctas, s)
+         : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.row_ctas, s) : launch_rows<T, D, 4>(p, pl.row_ctas, s);
   if (ce != cudaSuccess || p.direct) return ce;
-  p.splits = all;
   const long long rows = (long long)p.n_tokens * p.n_heads;
-  return launch(pattn::k_attn_join<T, D>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, p);
+  return launch(pattn::k_attn_join<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
 }
 
 // ------------------------------------------------------------------ sampling
@@ -359,8 +349,18 @@ extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void*
   p.v = pattn::Pages{c.v, c.v_page_stride, c.v_head_stride, c.v_slot_stride};
   p.prefix_pages = a.prefix_pages; p.page_table = a.page_table; p.suffix_lens = a.suffix_lens; p.cu_q = a.cu_q;
   p.table_stride = a.table_stride; p.status = a.status;
-  p.part_o = (float*)a.workspace;
-  p.part_ml = (float*)a.workspace + (size_t)(pl.tile_splits + pl.row_splits) * a.n_tokens * a.n_heads * c.head_dim;
+  float* ws = (float*)a.workspace;   // f32 rows first, so that they stay 16-byte aligned
+  p.tile_o = ws;
+  p.row_o = ws + pl.tile_rows * c.head_dim;
+  p.tile_ml = (float2*)(ws + (pl.tile_rows + pl.row_rows) * c.head_dim);
+  p.row_ml = p.tile_ml + pl.tile_rows;
+  p.row_parts = (int2*)(p.row_ml + pl.row_rows);
+  p.tile_parts = pl.tile_parts;
+  p.row_rows = (int)pl.row_rows;
+  p.rows_run = 8 * pl.nt;
+  p.own_only = pl.pairs > 0;
+  p.min_blocks = 2;
+  p.direct = !pl.nt && pl.tile_parts == 1;
   p.n_tokens = a.n_tokens; p.n_seqs = a.n_seqs; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads; p.group = a.n_heads / c.n_kv_heads;
   p.prefix_len = a.prefix_len; p.page_size = c.page_size; p.n_pages = c.n_pages; p.max_pages = a.max_pages;
   p.scale_log2 = a.scale * pattn::kLog2e;
