@@ -165,7 +165,9 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   __shared__ int s_items[kRowWarps], s_start_items, s_start_seq;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_launch();
-  griddep_wait();
+  // After the tile kernel, of which nothing is read here, this kernel starts on the SMs that it leaves
+  // free: the tile kernel lets it go only once what came before both is done.  It ends after it.
+  if (!p.tile_parts) griddep_wait();
 
   // ---- the line: its length, and the run of sequences in which this CTA's part begins
   const int n_chunks = (p.n_seqs + RUN - 1) / RUN;
@@ -185,7 +187,10 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   const long long warps = (long long)gridDim.x * kRowWarps;
   const long long per = max((total + warps - 1) / warps, (long long)p.min_blocks);
   const long long cta_first = (long long)blockIdx.x * kRowWarps * per;
-  if (cta_first >= total) return;
+  if (cta_first >= total) {
+    if (p.tile_parts) griddep_wait();
+    return;
+  }
   if (n_chunks > 1) {
     long long before = 0;
     int items = 0;
@@ -229,7 +234,10 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   const long long w_id = (long long)blockIdx.x * kRowWarps + warp;
   const long long u0 = w_id * per;
   long long u1 = min(total, u0 + per);
-  if (u0 >= total) return;                     // whole warps; no barrier follows
+  if (u0 >= total) {                           // whole warps; no barrier follows
+    if (p.tile_parts) griddep_wait();
+    return;
+  }
 
   // ---- the issuing side: where the warp stands in the line
   long long before = s_start;                  // units and items before sequence `chunk`
@@ -270,7 +278,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
         q.blocks = __shfl_sync(0xffffffffu, x.blocks, l);
         item_base = items + __shfl_sync(0xffffffffu, it_incl - it, l);
         const long long off = u - (before + __shfl_sync(0xffffffffu, incl - n, l));
-        in_item = (int)(off / q.blocks);
+        in_item = off <= 0x7fffffff ? (int)((unsigned)off / (unsigned)q.blocks) : (int)(off / q.blocks);
         blk = (int)(off - (long long)in_item * q.blocks);
         return;
       }
@@ -495,6 +503,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
     __syncwarp();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (p.tile_parts) griddep_wait();
 }
 
 // Tile `z` of a ragged grid: its sequence and the tile's number in it (warp-wide, all lanes).
@@ -551,12 +560,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
-// One row from shared to global memory; returns when the shared memory has been read.
-__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, int bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <typename T, int D, bool OWN>
@@ -602,8 +605,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
   }
-  griddep_launch();
   griddep_wait();
+  griddep_launch();   // the row kernel may start now: what came before is done
 
   // ---- the rows and keys of this CTA (the same in every thread)
   int b = 0, ti = blockIdx.x;
@@ -847,10 +850,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         const long long at = (long long)split * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
         if (live && !p.direct) p.tile_ml[at] = make_float2(m, l);
-        // rows to memory by one bulk copy each, staged in the ring (free now); 16 bytes of padding
-        // keep the threads' rows on different banks
-        const int row_bytes = p.direct ? D * 2 : D * 4;
-        uint8_t* stage = ring + (size_t)lr * (row_bytes + 16);
+        // Through the ring (free now), so that a warp writes whole rows; 16 bytes of padding keep the
+        // threads' rows on different banks
+        const int row_bytes = p.direct ? D * 2 : D * 4, pitch = row_bytes + 16;
+        uint8_t* stage = ring + (size_t)(wg * kTile + (warp & 3) * 32) * pitch;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           float o[32];
@@ -863,18 +866,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
           if (p.direct) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
-              *reinterpret_cast<uint4*>(stage + (c + i) * 2) =
+              *reinterpret_cast<uint4*>(stage + lane * pitch + (c + i) * 2) =
                   make_uint4(E::pack(o[i] * inv, o[i + 1] * inv), E::pack(o[i + 2] * inv, o[i + 3] * inv),
                              E::pack(o[i + 4] * inv, o[i + 5] * inv), E::pack(o[i + 6] * inv, o[i + 7] * inv));
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(stage + (c + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(stage + lane * pitch + (c + i) * 4) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
-        fence_async_smem();
-        if (live && (p.direct || m != -INFINITY)) {
-          void* dst = p.direct ? (void*)((T*)p.out + tok * p.o_tok + (long long)head * p.o_head) : (void*)(p.tile_o + at * D);
-          bulk_s2g(dst, smem_u32(stage), row_bytes);
+        __syncwarp();
+        const bool written = live && (p.direct || m != -INFINITY);
+        const long long dst = p.direct ? (tok * p.o_tok + (long long)head * p.o_head) * 2 : at * D * 4;
+        char* to = p.direct ? (char*)p.out : (char*)p.tile_o;
+        const unsigned all = __ballot_sync(0xffffffffu, written);
+        const int chunks = row_bytes / 16, rows_at_once = 32 / chunks;   // a warp writes 1, 2 or 4 rows at once
+        const int sub = lane / chunks, col = lane % chunks;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
+          const int r = r0 + sub;
+          const long long off = __shfl_sync(0xffffffffu, dst, r);
+          if (all >> r & 1) *reinterpret_cast<uint4*>(to + off + col * 16) = *reinterpret_cast<const uint4*>(stage + r * pitch + col * 16);
         }
       }
     }
@@ -890,8 +902,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
 
 // ---------------------------------------------------------------- joining key ranges
 // One warp per row (token, head): the maximum over its partials, then the weighted sums in the
-// order of the partials, so the result does not depend on timing.  Four weights and four partials are on their
-// way at a time.
+// order of the partials, so the result does not depend on timing.  Eight partials
+// are on their way at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Params p) {
   using E = ops::Elem<T>;
@@ -931,10 +943,10 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Param
       L += ml.y * f;
     }
     const int k = min(32, n - s0);
-    for (int s = 0; s < k; s += 4) {
-      float w[4], v[4][V];
+    for (int s = 0; s < k; s += 8) {
+      float w[8], v[8][V];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         w[j] = __shfl_sync(0xffffffffu, f, (s + j) & 31);
         if (s + j >= k) w[j] = 0.f;
 #pragma unroll
@@ -951,7 +963,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Param
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] += v[j][i] * w[j];
     }

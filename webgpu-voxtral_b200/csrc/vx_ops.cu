@@ -130,12 +130,13 @@ struct Plan {
 };
 
 // Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's
-// share of the key tiles least, a range's start and end counted as two tiles.
+// share of the key tiles least, a range's start and end (loading Q,
+// writing the partial) counted as four tiles.
 int tile_parts(long long items, long long tiles, int sms) {
   int best = 1;
   double least = 1e300;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 2.0);
+    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 4.0);
     if (cost < least * 0.999) {
       least = cost;
       best = s;
@@ -184,7 +185,9 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
     }
     if (own_keys || !pl.pairs) {
       pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
-      pl.row_ctas = sms;
+      // beside a tile kernel that leaves SMs free, those
+      const long long busy = pl.pairs * c.n_kv_heads * pl.tile_parts;
+      pl.row_ctas = busy <= sms / 2 ? (int)(sms - busy) : sms;
     }
   }
   const long long tile = 8 * pl.nt;
