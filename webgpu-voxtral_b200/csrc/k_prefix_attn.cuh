@@ -93,6 +93,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Barrier of `threads` threads that tells all of them whether one came with `v`.
+__device__ __forceinline__ bool named_bar_or(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(id), "r"(threads)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -537,16 +547,16 @@ __device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int 
 //   OWN = false: the rows of all sequences against the shared prefix, which is so read and
 //                multiplied once for the whole batch;
 //   OWN = true:  the rows of one sequence against its prefix and own keys, causally.
-// Warps 0-3 and 4-7 each do the softmax of one tile, a thread a row (no shuffles); warp 8 brings
-// the pages in by TMA; one thread of warp 9 issues the products.  While one tile's softmax runs,
-// the other tile's products do.  The reference exponent of a row only moves when its maximum grows
+// Warps 0-7 and 8-15 each do the softmax of one tile, two threads a row (64 keys each; no shuffles);
+// warp 16 brings the pages in by TMA; one thread of warp 17 issues the products.  While one tile's
+// softmax runs, the other tile's products do.  The reference exponent of a row only moves when its maximum grows
 // by more than 2^8 (weights stay below 2^8, far inside f16's and f32's range), so that O in TMEM is
 // hardly ever rescaled.
 //
 // Bound: for a wide batch the tensor cores and the exponentials (a 128 x 128 tile needs 1024 cycles
 // of products at head_dim 128 and 1024 of ex2), for a narrow one the reading of K and V.
 constexpr int kTile = 128;
-constexpr int kTileThreads = 320;
+constexpr int kTileThreads = 576;   // 16 warps of softmax, one that loads, one that multiplies
 template <int D>
 struct TileCfg {
   static constexpr int kSlot = kTile * D * 2;                       // a K or V tile, or a tile of Q
@@ -582,6 +592,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   uint64_t* p_full = s_full + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* tail = o_done + 1;
+  __shared__ float s_row[2][kTile];    // between the two threads of a row
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   volatile int* abort = &s_abort;
@@ -593,10 +604,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(q_full, 256);
+    mbar_init(q_full, 512);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], kTile);
+      mbar_init(&p_full[i], 2 * kTile);
     }
     mbar_init(o_done, 1);
     mbar_init(tail, 1);
@@ -632,14 +643,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   const int t0 = split * per, n = max(0, min(n_all, t0 + per) - t0);
   const int n_tiles = n_rows > kTile ? 2 : 1;
 
-  if (warp == 9) tc::tmem_alloc(&s_tmem, 512);
+  if (warp == 17) tc::tmem_alloc(&s_tmem, 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = s_tmem;
   const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 384};
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ---- pages into the ring: K of tile 0, V of tile 0, K of tile 1, ...
     const int box = min(p.page_size, kTile);
     int issued = 0, tails = 0;
@@ -692,7 +703,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     // after a failure nobody may be waiting for the last copies: they land before the CTA ends
     if (!ok || *abort)
       for (int it = max(0, issued - C::kSlots); it < issued; ++it) ops::wait_landed(&full[it % C::kSlots], (uint32_t)(it / C::kSlots) & 1u, p.status);
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     if (lane == 0 && n > 0) {
       const uint32_t q_s = smem_u32(smem), r_s = smem_u32(ring);
       const auto qk = [&](int i, int slot) {
@@ -736,21 +747,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       tc::tc_commit(o_done);
       if (!ok) ops::wait_landed(o_done, 0, p.status);   // products already issued end before TMEM is freed
     }
-  } else if (warp < 8) {
-    // ---- Q into shared memory (128-byte swizzle), then the softmax of one tile
-    const int wg = warp >> 2, row = threadIdx.x & (kTile - 1);
+  } else {
+    // ---- Q into shared memory (128-byte swizzle), then the softmax of half the keys of one tile
+    const int wg = warp >> 3, half = warp >> 2 & 1, row = threadIdx.x & (kTile - 1);
     {
-      constexpr int CH = D / 8, STEP = kTile / CH;   // 16-byte chunks of a row; this thread's rows are STEP apart
-      const int c = row % CH;
-      int g = (row0 + wg * kTile + row / CH) % p.group;
-      long long tok = tok0 + (row0 + wg * kTile + row / CH) / p.group;
+      constexpr int CH = D / 8, STEP = 2 * kTile / CH, N = CH / 2;   // 16-byte chunks of a row; this thread's rows are STEP apart
+      const int x = threadIdx.x & (2 * kTile - 1), c = x % CH, r0 = x / CH;
+      int g = (row0 + wg * kTile + r0) % p.group;
+      long long tok = tok0 + (row0 + wg * kTile + r0) / p.group;
       const int step_g = STEP % p.group, step_tok = STEP / p.group;
       const T* src = (const T*)p.q + (long long)kvh * p.group * p.q_head + c * 8;
-      uint4 v[CH];
+      uint4 v[N];
 #pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const bool in = wg * kTile + row / CH + k * STEP < n_rows;
-        v[k] = in ? *reinterpret_cast<const uint4*>(src + tok * p.q_tok + g * p.q_head) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < N; ++k) {
+        v[k] = wg * kTile + r0 + k * STEP < n_rows ? *reinterpret_cast<const uint4*>(src + tok * p.q_tok + g * p.q_head) : make_uint4(0, 0, 0, 0);
         g += step_g;
         tok += step_tok;
         if (g >= p.group) {
@@ -759,8 +769,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         }
       }
 #pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const int r = row / CH + k * STEP;
+      for (int k = 0; k < N; ++k) {
+        const int r = r0 + k * STEP;
         *reinterpret_cast<uint4*>(smem + wg * C::kSlot + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
       }
     }
@@ -768,70 +778,75 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     mbar_arrive(q_full);
 
     if (wg < n_tiles) {
+      constexpr int K = kTile / 2, DH = D / 2;
       const int lr = wg * kTile + row;   // this thread's row
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       const int lim = OWN ? first_lim + (row0 + min(lr, n_rows - 1)) / p.group : p.prefix_len;   // keys that the row sees
       float m = -INFINITY, l = 0.f;
+      // after a failed wait the threads of a tile go on to meet at the same barriers, without work
       bool ok = true;
       for (int j = 0; j < n; ++j) {
-        ok = ops::wait_phase(&s_full[wg], (uint32_t)j & 1u, abort, p.status, kDevTimeoutAcc);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        ok = __all_sync(0xffffffffu, ok && ops::wait_phase(&s_full[wg], (uint32_t)j & 1u, abort, p.status, kDevTimeoutAcc));
         tc::tc_fence_after();
-        float s[kTile];
-        tc::tmem_ld128(t_s[wg] + lanes, s);
+        float s[K];
+        tc::tmem_ld64(t_s[wg] + lanes + half * K, s);
         const int t = t0 + j;
         const bool pre = t < n_pre;
-        const int key = kTile * (pre ? t : t - n_pre);
-        const int see = min((pre ? p.prefix_len : own), lim - (pre ? 0 : p.prefix_len)) - key;   // keys of this tile that count
-        if (__any_sync(0xffffffffu, see < kTile)) {
+        const int key = kTile * (pre ? t : t - n_pre) + half * K;
+        const int see = min((pre ? p.prefix_len : own), lim - (pre ? 0 : p.prefix_len)) - key;   // keys of this half that count
+        if (__any_sync(0xffffffffu, see < K)) {
 #pragma unroll
-          for (int i = 0; i < kTile; ++i)
+          for (int i = 0; i < K; ++i)
             if (i >= see) s[i] = -INFINITY;
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i + 8 <= kTile; i += 8)
+        for (int i = 4; i + 8 <= K; i += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
-        mx[0] = max3(mx[0], s[kTile - 4], s[kTile - 3]);
-        mx[1] = max3(mx[1], s[kTile - 2], s[kTile - 1]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-        if (j == 0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
-          const float m_new = fmaxf(m, top), f = ex2(m == m_new ? 0.f : m - m_new);
+        mx[0] = max3(mx[0], s[K - 4], s[K - 3]);
+        mx[1] = max3(mx[1], s[K - 2], s[K - 1]);
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        // The two halves' scores are in registers once all have met here, so the weights may take
+        // their columns; and all know whether a row of the tile has outgrown its reference
+        tc::tc_fence_before();
+        if (named_bar_or(1 + wg, 2 * kTile, j == 0 || top > m + 8.f)) {
+          if (half == 1) s_row[wg][row] = top;
+          named_bar_sync(1 + wg, 2 * kTile);
+          if (half == 0) s_row[wg][row] = fmaxf(m, fmaxf(top, s_row[wg][row]));
+          named_bar_sync(1 + wg, 2 * kTile);
+          const float m_new = s_row[wg][row], f = m == m_new ? 1.f : ex2(m - m_new);
           l *= f;
           m = m_new;
+          tc::tc_fence_after();
+          if (j > 0) {
+            // scores in TMEM mean that the products before them are done: O may change
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
-            float o[16];
-            uint32_t u[16];
-            tc::tmem_ld16(t_o[wg] + lanes + c, o);
+            for (int c = half * DH; c < (half + 1) * DH; c += 16) {
+              float o[16];
+              uint32_t u[16];
+              tc::tmem_ld16(t_o[wg] + lanes + c, o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f);
-            tc::tmem_st16(t_o[wg] + lanes + c, u);
+              for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(o[i] * f);
+              tc::tmem_st16(t_o[wg] + lanes + c, u);
+            }
           }
         }
+        tc::tc_fence_after();
         const float m_use = m == -INFINITY ? 0.f : m;
         const f32x2 scale2 = pack2(p.scale_log2, p.scale_log2), off2 = pack2(-m_use, -m_use);
         f32x2 sum[2] = {pack2(l, 0.f), pack2(0.f, 0.f)};
+        uint32_t u[K / 2];
 #pragma unroll
-        for (int c = 0; c < kTile; c += 64) {
-          uint32_t u[32];
-#pragma unroll
-          for (int i = 0; i < 64; i += 2) {
-            float x, y;
-            unpack2(fma2(pack2(s[c + i], s[c + i + 1]), scale2, off2), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(x, y));
-            u[i >> 1] = E::pack(x, y);
-          }
-          tc::tmem_st32(t_s[wg] + lanes + c / 2, u);
+        for (int i = 0; i < K; i += 2) {
+          float x, y;
+          unpack2(fma2(pack2(s[i], s[i + 1]), scale2, off2), x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(x, y));
+          u[i >> 1] = E::pack(x, y);
         }
+        tc::tmem_st32(t_s[wg] + lanes + half * (K / 2), u);
         {
           float x, y;
           unpack2(add2(sum[0], sum[1]), x, y);
@@ -841,7 +856,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         tc::tc_fence_before();
         mbar_arrive(&p_full[wg]);
       }
-      if (ok && n > 0) ok = __all_sync(0xffffffffu, ops::wait_phase(o_done, 0, abort, p.status, kDevTimeoutAcc));
+      if (n > 0) ok = __all_sync(0xffffffffu, ok && ops::wait_phase(o_done, 0, abort, p.status, kDevTimeoutAcc));
+      named_bar_sync(1 + wg, 2 * kTile);       // the last maxima are read
+      if (half == 1) s_row[wg][row] = l;
+      named_bar_sync(1 + wg, 2 * kTile);
+      if (half == 0) s_row[wg][row] = l + s_row[wg][row];
+      named_bar_sync(1 + wg, 2 * kTile);
+      l = s_row[wg][row];
       if (ok) {
         tc::tc_fence_after();
         const bool live = lr < n_rows;
@@ -849,16 +870,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         const int head = kvh * p.group + (row0 + lr) % p.group;
         const long long at = (long long)split * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        if (live && !p.direct) p.tile_ml[at] = make_float2(m, l);
-        // Through the ring (free now), so that a warp writes whole rows; 16 bytes of padding keep the
-        // threads' rows on different banks
-        const int row_bytes = p.direct ? D * 2 : D * 4, pitch = row_bytes + 16;
-        uint8_t* stage = ring + (size_t)(wg * kTile + (warp & 3) * 32) * pitch;
+        if (live && !p.direct && half == 0) p.tile_ml[at] = make_float2(m, l);
+        // Through the ring (free now), so that a warp writes whole halves of rows; 16 bytes of padding
+        // keep the threads' rows on different banks
+        const int row_bytes = p.direct ? DH * 2 : DH * 4, pitch = row_bytes + 16;
+        uint8_t* stage = ring + (size_t)warp * 32 * pitch;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = 0; c < DH; c += 32) {
           float o[32];
           if (n > 0) {
-            tc::tmem_ld32(t_o[wg] + lanes + c, o);
+            tc::tmem_ld32(t_o[wg] + lanes + half * DH + c, o);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
@@ -877,10 +898,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
         }
         __syncwarp();
         const bool written = live && (p.direct || m != -INFINITY);
-        const long long dst = p.direct ? (tok * p.o_tok + (long long)head * p.o_head) * 2 : at * D * 4;
+        const long long dst = p.direct ? (tok * p.o_tok + (long long)head * p.o_head + half * DH) * 2 : (at * D + half * DH) * 4;
         char* to = p.direct ? (char*)p.out : (char*)p.tile_o;
         const unsigned all = __ballot_sync(0xffffffffu, written);
-        const int chunks = row_bytes / 16, rows_at_once = 32 / chunks;   // a warp writes 1, 2 or 4 rows at once
+        const int chunks = row_bytes / 16, rows_at_once = 32 / chunks;   // a warp writes 2, 4 or 8 half rows at once
         const int sub = lane / chunks, col = lane % chunks;
 #pragma unroll 4
         for (int r0 = 0; r0 < 32; r0 += rows_at_once) {
@@ -894,7 +915,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   __syncwarp();
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
