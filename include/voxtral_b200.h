@@ -428,9 +428,10 @@ int vx_shared_prefix_attention(const vx_shared_prefix_args* a, void* stream, cha
  * mass reaches top_p of what is left (1 or more: all; at least one token); the token is the
  * first whose running mass reaches u * (kept mass), u in [0, 1).  With top_k 0 and min_p 0 this is
  * the order and rule of sampleTopP (src/engine.ts:247-289), masses in f64.  temperature <= 0: the
- * first of the largest.  out[r]: the index, -1 for a row without a finite or +inf logit.
- * Each setting is a device array by row, or (array null) the value beside it for all rows.
- * n_cols <= 262144. */
+ * first of the largest (values above 1e30 count as 1e30).  out[r]: the index, -1 for a row without
+ * a finite or +inf logit (NaN counts as -inf; where there is +inf, those tokens alone are drawn).
+ * Each setting is a device array by row, or (array null) the value beside it for all rows, with
+ * the same result as an array of that value.  n_cols <= 262144. */
 typedef struct vx_sample_args {
   const void* logits;
   const double* u; /* [n_rows] */
@@ -438,10 +439,10 @@ typedef struct vx_sample_args {
   const int32_t* top_k;
   int32_t* out;
   int64_t row_stride;
-  double temperature_all, top_p_all, min_p_all;
+  float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   int32_t dtype; /* F16, BF16 or F32 */
-  int32_t n_rows, n_cols, reserved[2];
+  int32_t n_rows, n_cols, reserved;
 } vx_sample_args;
 int vx_sample_logits(const vx_sample_args* a, void* stream, char* err, size_t err_len);
 

@@ -357,7 +357,8 @@ def sample_reference(row, u, temperature, top_k, top_p, min_p):
 def check_sample(vx, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     got = vx.sample_logits(logits, torch.from_numpy(u).cuda(), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p).cpu().numpy()
     host = logits.double().cpu().numpy()
-    each = [v.cpu().numpy() if torch.is_tensor(v) else [v] * len(u) for v in (temperature, top_k, top_p, min_p)]
+    # a number counts as an f32 array of that value
+    each = [v.cpu().numpy() if torch.is_tensor(v) else [np.float32(v)] * len(u) for v in (temperature, top_k, top_p, min_p)]
     for r in range(len(u)):
         want, slack = sample_reference(host[r], u[r], float(each[0][r]), int(each[1][r]), float(each[2][r]), float(each[3][r]))
         assert slack > 0 or u[r] == 0, r
@@ -427,6 +428,13 @@ def test_sample_strides_and_out(vx):
     assert vx.sample_logits(big[0, :0], u[:0]).shape == (0,)
 
 
+def test_sample_numbers_are_arrays_of_one_value(vx):
+    x, u = rand(64, 131072, seed=12, scale=1.5), torch.rand(64, dtype=torch.float64, device="cuda")
+    full = [torch.full((64,), v, device="cuda") for v in (0.8, 0.95, 0.001)]
+    a = vx.sample_logits(x, u, temperature=0.8, top_p=0.95, min_p=0.001)
+    assert torch.equal(a, vx.sample_logits(x, u, temperature=full[0], top_p=full[1], min_p=full[2]))
+
+
 def test_sample_follows_the_distribution(vx):
     """20000 draws of one row: counts within 6 standard deviations of the kept masses."""
     x = torch.tensor([1.0, 0.5, 2.0, -1.0, 0.0, -30.0], device="cuda")
@@ -477,7 +485,7 @@ class Step:
         want, tol = attend_reference(q, self.kp, self.vp, self.ppages, self.prefix, self.table, lens, self.d ** -0.5)
         assert torch.all((o.double() - want).abs() <= tol)
         for r in range(len(lens)):
-            idx, slack = sample_reference(logits[r].double().cpu().numpy(), float(self.u[r]), 0.9, 300, 0.97, 0.0)
+            idx, slack = sample_reference(logits[r].double().cpu().numpy(), float(self.u[r]), float(np.float32(0.9)), 300, float(np.float32(0.97)), 0.0)
             assert slack > 0 and int(tok[r]) == idx
 
 

@@ -191,7 +191,7 @@ def test_attend_c_refuses(ops, cache, change, code, word):
     (dict(rows=0), 0, ""),
 ])
 def test_sample_c_refuses(ops, change, code, word):
-    a = dict(logits=P, u=P, tp=0, topp=0, minp=0, topk=0, out=P, stride=9, t=1.0, top_p=1.0, min_p=0.0, k=0, dtype=0, rows=2, n=9, r0=0, r1=0)
+    a = dict(logits=P, u=P, tp=0, topp=0, minp=0, topk=0, out=P, stride=9, t=1.0, top_p=1.0, min_p=0.0, k=0, dtype=0, rows=2, n=9, reserved=0)
     a.update(change)
     rc, msg = _c(ops, "vx_sample_logits", ops._SAMPLE.pack(*a.values()))
     assert rc == code and word in msg, (rc, msg)

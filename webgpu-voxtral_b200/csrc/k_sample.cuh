@@ -58,7 +58,7 @@ struct Params {
   const double* u;
   const float *temperature, *top_p, *min_p;   // by row, or null: the value below for every row
   const int32_t* top_k;
-  double temperature1, top_p1, min_p1;
+  float temperature1, top_p1, min_p1;
   int top_k1;
   int32_t* out;
   int n, slice;
@@ -698,10 +698,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   }
 
   Row r;
-  double temp = p.temperature ? (double)p.temperature[row] : p.temperature1;
+  double temp = (double)(p.temperature ? p.temperature[row] : p.temperature1);
   int k = p.top_k ? p.top_k[row] : p.top_k1;
-  const double top_p = p.top_p ? (double)p.top_p[row] : p.top_p1;
-  const double min_p = fmin(1.0, p.min_p ? (double)p.min_p[row] : p.min_p1);
+  const double top_p = (double)(p.top_p ? p.top_p[row] : p.top_p1);
+  const double min_p = fmin(1.0, (double)(p.min_p ? p.min_p[row] : p.min_p1));
   const double u = p.u[row];
   if (!(temp > 0.0)) {   // greedy
     temp = 1.0;

@@ -382,11 +382,11 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   if (a.dtype < 0 || a.dtype > 2) return e.fail(VX_E_INVALID, "dtype %d (0 F16, 1 BF16, 2 F32)", a.dtype);
   if (a.n_rows < 0 || a.n_cols < 1 || a.n_cols > most || a.row_stride < 0)
     return e.fail(VX_E_RANGE, "%d rows of %d logits (1 to %d), stride %lld", a.n_rows, a.n_cols, most, (long long)a.row_stride);
-  if (!a.temperature && !(a.temperature_all >= 0.0 && a.temperature_all <= 3e38))
-    return e.fail(VX_E_RANGE, "temperature %g must be 0 or more", a.temperature_all);
-  if (!a.top_p && !(a.top_p_all >= 0.0)) return e.fail(VX_E_RANGE, "top_p %g must be 0 or more", a.top_p_all);
-  if (!a.min_p && !(a.min_p_all >= 0.0 && a.min_p_all <= 1.0))
-    return e.fail(VX_E_RANGE, "min_p %g must be in [0, 1]", a.min_p_all);
+  if (!a.temperature && !(a.temperature_all >= 0.f && a.temperature_all <= 3e38f))
+    return e.fail(VX_E_RANGE, "temperature %g must be 0 or more", (double)a.temperature_all);
+  if (!a.top_p && !(a.top_p_all >= 0.f)) return e.fail(VX_E_RANGE, "top_p %g must be 0 or more", (double)a.top_p_all);
+  if (!a.min_p && !(a.min_p_all >= 0.f && a.min_p_all <= 1.f))
+    return e.fail(VX_E_RANGE, "min_p %g must be in [0, 1]", (double)a.min_p_all);
   if (a.n_rows == 0) return e.ok();
   if (!a.logits || !a.u || !a.out) return e.fail(VX_E_INVALID, "logits, u and out must be device pointers");
   if (reinterpret_cast<uintptr_t>(a.logits) % elem_size(a.dtype)) return e.fail(VX_E_INVALID, "logits must be aligned to their type");

@@ -47,8 +47,8 @@ koffi.struct('vx_shared_prefix_args', {
 });
 koffi.struct('vx_sample_args', {
   logits: 'void *', u: 'void *', temperature: 'void *', top_p: 'void *', min_p: 'void *', top_k: 'void *', out: 'void *',
-  row_stride: 'int64', temperature_all: 'double', top_p_all: 'double', min_p_all: 'double', top_k_all: 'int32',
-  dtype: 'int32', n_rows: 'int32', n_cols: 'int32', reserved: koffi.array('int32', 2),
+  row_stride: 'int64', temperature_all: 'float', top_p_all: 'float', min_p_all: 'float', top_k_all: 'int32',
+  dtype: 'int32', n_rows: 'int32', n_cols: 'int32', reserved: 'int32',
 });
 
 // One entry per declaration of include/voxtral_b200.h.

@@ -32,7 +32,7 @@ _INT = torch.int32
 _CACHE = "2P6q6i"                                # vx_kv_pages
 _APPEND = struct.Struct("@" + _CACHE + "4P8q5Pq8i")   # vx_rope_append_args
 _PREFIX = struct.Struct("@" + _CACHE + "2P4q6P2q5if")  # vx_shared_prefix_args
-_SAMPLE = struct.Struct("@7Pq3d6i")              # vx_sample_args
+_SAMPLE = struct.Struct("@7Pq3f5i")              # vx_sample_args
 _ERR = 256
 _local = threading.local()
 
@@ -242,7 +242,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     min_p drops what is less likely than min_p times the first, top_k keeps that many (0: all), top_p
     the shortest run that holds that share of the remaining mass; the token is the first whose
     running mass reaches u times the kept mass.  temperature 0 takes the first.  Each setting is a
-    number, or a tensor by row (f32; top_k int32).  Returns int32 [n_rows]; -1 for a row whose
+    tensor by row (f32; top_k int32), or a number, which counts as such a tensor of that value.  Returns int32 [n_rows]; -1 for a row whose
     logits are all -inf or NaN."""
     shape, stride = _rows("logits", logits, 2, *_DTYPE)
     rows, cols = shape
@@ -270,5 +270,5 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     device = _same_place("logits u setting setting setting setting out", *tensors)
     _call(_library().vx_sample_logits,
           _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), stride[0], one[0], one[1], one[2], int(one[3]),
-                       _DTYPE[logits.dtype], rows, cols, 0, 0), device)
+                       _DTYPE[logits.dtype], rows, cols, 0), device)
     return out
