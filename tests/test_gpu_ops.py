@@ -242,6 +242,13 @@ ATTEND = [  # lens, prefix, heads, kv, dim, page, type, token_major
     ([(33, 290), (0, 0), (1, 1), (260, 260)], 0, 6, 3, 128, 16, F16, False),
     ([(600, 600)], 64, 7, 7, 64, 64, BF16, False),
     ([(40, 47), (90, 95)], 515, 40, 2, 128, 128, F16, False),
+    # ragged rows that take a long prefix together, then their own keys by rows or by tiles
+    ([(1 + 7 * i % 41, 1 + 7 * i % 41 + 13 * i % 50) for i in range(14)], 3001, 32, 8, 128, 64, F16, False),
+    ([(1 + 5 * i % 30, 3 * i % 17) for i in range(30)], 2600, 24, 8, 64, 16, BF16, True),   # some stand inside the prefix
+    ([(90, 101), (70, 70), (0, 3), (83, 200), (100, 50)], 2300, 32, 8, 128, 32, BF16, False),
+    ([(3, 0), (64, 0), (1, 0), (20, 0)], 4000, 32, 8, 128, 128, F16, False),               # no own keys at all
+    ([(1, 1 + i % 3) for i in range(400)], 0, 8, 8, 128, 16, F16, False),                    # many short sequences
+    ([(1, 0 if i % 7 else 40) for i in range(500)], 300, 16, 4, 64, 16, BF16, False),
 ]
 
 

@@ -45,7 +45,9 @@ struct Params {
   int tile_parts;            // key ranges of the tile kernel (0: it does not run)
   int row_rows;              // partial rows there is room for
   int rows_run;              // whether the row kernel runs, and the rows of its tiles
-  int own_only;              // the row kernel leaves the prefix to the tile kernel
+  int own_only;              // the prefix is the shared tile kernel's: the row kernel and the one of whole sequences leave it out
+  int part0;                 // this tile launch's first partial
+  int parts;                 // and its key ranges
   int min_blocks;            // blocks a warp of the row kernel takes at least
   int direct;                // the tile kernel alone, with one key range: it writes out
 };
@@ -122,6 +124,7 @@ __device__ __forceinline__ float ex2(float x) {
 //
 // Bound: the reading of K and V (HBM, or L2 where sequences read the same prefix).
 constexpr int kRowStages = 3;
+constexpr int kItemCost = 1;
 // Warps of a CTA, one CTA an SM: as many as shared memory holds rings for (registers allow them too).
 constexpr int row_warps(int d, int nt) {
   return d == 128 ? (nt == 1 ? 7 : nt == 2 ? 6 : 4) : (nt == 1 ? 14 : nt == 2 ? 12 : 8);
@@ -138,7 +141,10 @@ constexpr int row_smem() {
 // A sequence as the row kernel sees it.
 struct Seq {
   int tok0, nq, own, tiles, blocks;   // query tokens, own keys, row tiles, 16-key blocks (prefix and own)
-  __device__ __forceinline__ long long units(int n_kv) const { return (long long)tiles * n_kv * blocks; }
+  // An item counts kItemCost blocks more than it has: what its start (q, page numbers) and its end (a
+  // partial) take.  Otherwise the warps whose share is many short sequences are the last to be done.
+  __device__ __forceinline__ int item_units() const { return blocks ? blocks + kItemCost : 0; }
+  __device__ __forceinline__ long long units(int n_kv) const { return (long long)tiles * n_kv * item_units(); }
 };
 __device__ __forceinline__ Seq sequence(const Params& p, int b, int rows) {
   Seq q{0, 0, 0, 0, 0};
@@ -253,7 +259,8 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   long long before = s_start;                  // units and items before sequence `chunk`
   int items = s_start_items, chunk = s_start_seq;
   Seq q{};
-  int b = 0, in_item = 0, blk = 0, part_left = 0, q_count = 0, page_lane = 0, page_from = 0;
+  int issued = 0, done = 0;                    // blocks
+  int b = -1, in_item = 0, blk = 0, part_left = 0, q_count = 0, page_lane = 0, page_from = 0;
   bool part_starts = false;
   long long u = u0;
   uint8_t* mine = smem + warp * row_warp_smem<D, NT>();
@@ -288,8 +295,9 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
         q.blocks = __shfl_sync(0xffffffffu, x.blocks, l);
         item_base = items + __shfl_sync(0xffffffffu, it_incl - it, l);
         const long long off = u - (before + __shfl_sync(0xffffffffu, incl - n, l));
-        in_item = off <= 0x7fffffff ? (int)((unsigned)off / (unsigned)q.blocks) : (int)(off / q.blocks);
-        blk = (int)(off - (long long)in_item * q.blocks);
+        const int iu = q.item_units();
+        in_item = off <= 0x7fffffff ? (int)((unsigned)off / (unsigned)iu) : (int)(off / iu);
+        blk = (int)(off - (long long)in_item * iu) - kItemCost;   // below 0: before the item's first block
         return;
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
@@ -303,31 +311,38 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   };
   const int pre_blocks = p.own_only ? 0 : (p.prefix_len + 15) / 16;
   const auto issue = [&](int st) {
-    if (u < u1) {
-      if (part_left == 0) {                    // the next part: the rest of this item, or of this warp's units
-        if (u == u0 || in_item + 1 >= q.tiles * p.n_kv) {
-          locate();
-        } else {
-          ++in_item;
-          blk = 0;
-        }
-        part_left = (int)min((long long)(q.blocks - blk), u1 - u);
-        part_starts = true;
-        page_from = -64;
+    while (u < u1 && part_left == 0) {         // the next part: the rest of this item, or of this warp's units
+      if (u == u0 || in_item + 1 >= q.tiles * p.n_kv) {
+        const int was = b;
+        locate();
+        if (b != was || u == u0) page_from = -64;
+      } else {
+        ++in_item;
+        blk = -kItemCost;
       }
+      if (blk < 0) {                           // the item's cost before its first block
+        const int skip = (int)min((long long)-blk, u1 - u);
+        blk += skip;
+        u += skip;
+      }
+      if (blk < 0 || u >= u1) break;
+      part_left = (int)min((long long)(q.blocks - blk), u1 - u);
+      part_starts = true;
+    }
+    {
       if (u < u1) {
         const int ti = in_item / p.n_kv, kvh = in_item - ti * p.n_kv;
         const bool pre = blk < pre_blocks;
         const int key = 16 * (pre ? blk : blk - pre_blocks);
         const int keys = (pre ? p.prefix_len : q.own) - key;
         // page numbers of 32 blocks at once, a block a lane
-        if (blk - page_from >= 32) {
+        if (blk < page_from || blk - page_from >= 32) {
           page_from = blk;
           const int bl = blk + lane;
           const bool bp = bl < pre_blocks;
           const int lp = 16 * (bp ? bl : bl - pre_blocks) / p.page_size;
           page_lane = -1;
-          if (bl < blk + part_left) {
+          if (bl < q.blocks) {
             if (bp) page_lane = p.prefix_pages[lp];
             else if (lp < p.max_pages) page_lane = p.page_table[(long long)b * p.table_stride + lp];
             if (page_lane < 0 || page_lane >= p.n_pages) {
@@ -370,6 +385,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
         ++blk;
         --part_left;
         ++u;
+        ++issued;
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -382,7 +398,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   for (int s = 0; s < kRowStages - 1; ++s) issue(s);
   int st = 0;
   bool item_first = false;                     // the warp's part holds the item's first block
-  for (long long i = u0; i < u1; ++i) {
+  for (; done < issued; ++done) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
     __syncwarp();
     const Stage sg = stages[st];
@@ -637,9 +653,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     n_rows = min((long long)2 * kTile, (long long)p.n_tokens * p.group - (long long)ti * 2 * kTile);
   }
   const int row0 = ti * 2 * kTile;                       // first row: token tok0 + row / group, head row % group
-  const int n_pre = (min(p.prefix_len, last_lim) + kTile - 1) / kTile;
+  const int n_pre = OWN && p.own_only ? 0 : (min(p.prefix_len, last_lim) + kTile - 1) / kTile;
   const int n_all = n_pre + (max(0, last_lim - p.prefix_len) + kTile - 1) / kTile;
-  const int per = (n_all + p.tile_parts - 1) / p.tile_parts;
+  const int per = (n_all + p.parts - 1) / p.parts;
   const int t0 = split * per, n = max(0, min(n_all, t0 + per) - t0);
   const int n_tiles = n_rows > kTile ? 2 : 1;
 
@@ -781,7 +797,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       constexpr int K = kTile / 2, DH = D / 2;
       const int lr = wg * kTile + row;   // this thread's row
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const int lim = OWN ? first_lim + (row0 + min(lr, n_rows - 1)) / p.group : p.prefix_len;   // keys that the row sees
+      int lim = OWN ? first_lim + (row0 + min(lr, n_rows - 1)) / p.group : p.prefix_len;   // keys that the row sees
+      if (!OWN && p.cu_q) {
+        // the row's sequence: where its queries reach into the prefix, they do not see all of it
+        const int tok = (row0 + min(lr, n_rows - 1)) / p.group;
+        int lo = 0, hi = p.n_seqs;             // cu_q[lo] <= tok < cu_q[hi], if it is any sequence's
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (p.cu_q[mid] <= tok) lo = mid;
+          else hi = mid;
+        }
+        const int own_keys = max(0, min(p.suffix_lens[lo], p.max_pages * p.page_size));
+        lim = min(p.prefix_len, p.prefix_len + own_keys - p.cu_q[lo + 1] + tok + 1);
+      }
       float m = -INFINITY, l = 0.f;
       // after a failed wait the threads of a tile go on to meet at the same barriers, without work
       bool ok = true;
@@ -865,10 +893,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       l = s_row[wg][row];
       if (ok) {
         tc::tc_fence_after();
-        const bool live = lr < n_rows;
         const long long tok = tok0 + (row0 + lr) / p.group;
+        const bool live = lr < n_rows && (OWN || !p.cu_q || (tok >= p.cu_q[0] && tok < p.cu_q[p.n_seqs]));
         const int head = kvh * p.group + (row0 + lr) % p.group;
-        const long long at = (long long)split * p.n_tokens * p.n_heads + tok * p.n_heads + head;
+        const long long at = (long long)(p.part0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
         if (live && !p.direct && half == 0) p.tile_ml[at] = make_float2(m, l);
         // Through the ring (free now), so that a warp writes whole halves of rows; 16 bytes of padding

@@ -120,12 +120,13 @@ cudaError_t launch_append(const append::Params& p, int interleaved, cudaStream_t
 
 // ------------------------------------------------------------------ attention
 struct Plan {
-  int own;              // tile kernel over prefix and own keys (1) or the shared prefix alone (0)
-  long long pairs;      // tile kernel: pairs of 128-row tiles; 0: not launched
-  int tile_parts;
-  int nt;               // row kernel: tiles of 8 nt rows; 0: not launched
+  long long shared_pairs;   // tile kernel of all rows over the shared prefix: pairs of 128-row tiles; 0: not launched
+  int shared_parts;
+  long long own_pairs;      // tile kernel of each sequence's rows over its keys; 0: not launched
+  int own_parts;
+  int nt;                   // row kernel: tiles of 8 nt rows; 0: not launched
   int row_ctas;
-  int64_t tile_rows, row_rows;   // partial rows of each kernel
+  int64_t tile_rows, row_rows;   // partial rows of each kind
   int64_t bytes;
 };
 
@@ -170,31 +171,35 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
   const long long own_keys = (long long)a.max_pages * c.page_size, rows = (long long)a.n_tokens * group;
   pl = Plan{};
-  // The tile kernel multiplies 128 rows at once; below 64 rows a sequence the row kernel's tiles
-  // of 32 waste less.
-  pl.own = a.cu_q && rows >= 64ll * a.n_seqs;
-  if (pl.own) {
-    pl.pairs = rows / 256 + a.n_seqs;
-    pl.tile_parts = tile_parts(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128 + (own_keys + 127) / 128, sms);
-  } else {
-    // One token a sequence: all sequences' rows take the prefix together in the tile kernel, where
-    // reading it for each of them (from L2, 8 MB a us) would take longer than that kernel's start and end
-    if (!a.cu_q && (double)a.n_seqs * a.prefix_len * c.n_kv_heads * c.head_dim * 4 > kSharePrefixBytes) {
-      pl.pairs = (rows + 255) / 256;
-      pl.tile_parts = tile_parts(pl.pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
-    }
-    if (own_keys || !pl.pairs) {
-      pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
-      // beside a tile kernel that leaves SMs free, those
-      const long long busy = pl.pairs * c.n_kv_heads * pl.tile_parts;
-      pl.row_ctas = busy <= sms / 2 ? (int)(sms - busy) : sms;
-    }
+  const long long each = rows / std::max(1, a.n_seqs);   // rows a sequence
+  // The row kernel reads the prefix again for every sequence (every 32 rows of one): from L2, 8 MB a us.
+  // Where that would take longer than the tile kernel's start and end, the rows of all sequences
+  // take the prefix together; not where the sequences' rows fill tiles by themselves, and partials of
+  // the prefix and of the own keys would only add to the work.
+  const double again = (double)(a.cu_q ? rows / 32 + a.n_seqs : a.n_seqs) * a.prefix_len * c.n_kv_heads * c.head_dim * 4;
+  if (a.n_seqs > 1 && again > kSharePrefixBytes && each < 512) {
+    pl.shared_pairs = (rows + 255) / 256;
+    pl.shared_parts = tile_parts(pl.shared_pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
+  }
+  // The tile kernel multiplies 128 rows at once; of sequences with fewer than 64 (256 for the own keys
+  // alone, of which there are fewer) the row kernel's tiles of 32 waste less
+  if (a.cu_q && own_keys + a.prefix_len && each >= (pl.shared_pairs ? 256 : 64)) {
+    pl.own_pairs = rows / 256 + a.n_seqs;
+    const long long keys = (pl.shared_pairs ? 0 : (a.prefix_len + 127) / 128) + (own_keys + 127) / 128;
+    pl.own_parts = keys ? tile_parts(pl.own_pairs * c.n_kv_heads, keys, sms) : 0;
+    if (!keys) pl.own_pairs = 0;
+  } else if (own_keys || !pl.shared_pairs) {
+    pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
+    // beside a tile kernel that leaves SMs free, those
+    const long long busy = pl.shared_pairs * c.n_kv_heads * pl.shared_parts;
+    pl.row_ctas = busy <= sms / 2 ? (int)(sms - busy) : sms;
   }
   const long long tile = 8 * pl.nt;
   const long long items = !pl.nt ? 0 : (a.cu_q ? rows / tile + a.n_seqs : a.n_seqs * ((group + tile - 1) / tile)) * c.n_kv_heads;
-  pl.tile_rows = pl.pairs && (pl.nt || pl.tile_parts > 1) ? (int64_t)pl.tile_parts * a.n_tokens * a.n_heads : 0;
+  const int parts = pl.shared_parts + pl.own_parts;
+  pl.tile_rows = pl.nt || parts > 1 ? (int64_t)parts * a.n_tokens * a.n_heads : 0;
   pl.row_rows = pl.nt ? ((int64_t)pl.row_ctas * pattn::row_warps(c.head_dim, pl.nt) + items) * tile : 0;
-  if (pl.pairs > 0x7fffffff || pl.row_rows > 0x7fffffff || (long long)a.n_tokens * a.n_heads > 0x7fffffff)
+  if (std::max(pl.shared_pairs, pl.own_pairs) > 0x7fffffff || pl.row_rows > 0x7fffffff || (long long)a.n_tokens * a.n_heads > 0x7fffffff)
     return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
   pl.bytes = (pl.tile_rows + pl.row_rows) * (c.head_dim + 2) * 4 + (pl.nt ? (int64_t)a.n_tokens * a.n_heads * 8 : 0);
   return VX_OK;
@@ -236,7 +241,9 @@ cudaError_t launch_rows(const pattn::Params& p, int ctas, cudaStream_t s) {
   return launch(pattn::k_attn_rows<T, D, NT>, dim3(ctas), dim3(pattn::row_warps(D, NT) * 32), bytes, s, p);
 }
 template <typename T, int D, bool OWN>
-cudaError_t launch_tiles(const pattn::Params& p, const vx_kv_pages& c, long long pairs, cudaStream_t s) {
+cudaError_t launch_tiles(pattn::Params p, const vx_kv_pages& c, long long pairs, int part0, int parts, cudaStream_t s) {
+  p.part0 = part0;
+  p.parts = parts;
   static std::atomic<int> done[kMaxDevices];
   constexpr size_t bytes = pattn::TileCfg<D>::kSmem;
   cudaError_t ce = allow_smem(pattn::k_attn_tiles<T, D, OWN>, done, bytes);
@@ -244,13 +251,14 @@ cudaError_t launch_tiles(const pattn::Params& p, const vx_kv_pages& c, long long
   if (ce == cudaSuccess) ce = encode_pages(&km, c, p.k);
   if (ce == cudaSuccess) ce = encode_pages(&vm, c, p.v);
   if (ce != cudaSuccess) return ce;
-  return launch(pattn::k_attn_tiles<T, D, OWN>, dim3((unsigned)pairs, p.n_kv, p.tile_parts), dim3(pattn::kTileThreads), bytes, s, km, vm, p);
+  return launch(pattn::k_attn_tiles<T, D, OWN>, dim3((unsigned)pairs, p.n_kv, parts), dim3(pattn::kTileThreads), bytes, s, km, vm, p);
 }
 
 template <typename T, int D>
 cudaError_t launch_attention(const pattn::Params& p, const vx_kv_pages& c, const Plan& pl, cudaStream_t s) {
   cudaError_t ce = cudaSuccess;
-  if (pl.pairs) ce = pl.own ? launch_tiles<T, D, true>(p, c, pl.pairs, s) : launch_tiles<T, D, false>(p, c, pl.pairs, s);
+  if (pl.shared_pairs) ce = launch_tiles<T, D, false>(p, c, pl.shared_pairs, 0, pl.shared_parts, s);
+  if (ce == cudaSuccess && pl.own_pairs) ce = launch_tiles<T, D, true>(p, c, pl.own_pairs, pl.shared_parts, pl.own_parts, s);
   if (ce == cudaSuccess && pl.nt)
     ce = pl.nt == 1 ? launch_rows<T, D, 1>(p, pl.row_ctas, s)
          : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.row_ctas, s) : launch_rows<T, D, 4>(p, pl.row_ctas, s);
@@ -358,12 +366,12 @@ extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void*
   p.tile_ml = (float2*)(ws + (pl.tile_rows + pl.row_rows) * c.head_dim);
   p.row_ml = p.tile_ml + pl.tile_rows;
   p.row_parts = (int2*)(p.row_ml + pl.row_rows);
-  p.tile_parts = pl.tile_parts;
+  p.tile_parts = pl.shared_parts + pl.own_parts;
   p.row_rows = (int)pl.row_rows;
   p.rows_run = 8 * pl.nt;
-  p.own_only = pl.pairs > 0;
+  p.own_only = pl.shared_pairs > 0;
   p.min_blocks = 2;
-  p.direct = !pl.nt && pl.tile_parts == 1;
+  p.direct = !pl.nt && p.tile_parts == 1;
   p.n_tokens = a.n_tokens; p.n_seqs = a.n_seqs; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads; p.group = a.n_heads / c.n_kv_heads;
   p.prefix_len = a.prefix_len; p.page_size = c.page_size; p.n_pages = c.n_pages; p.max_pages = a.max_pages;
   p.scale_log2 = a.scale * pattn::kLog2e;
