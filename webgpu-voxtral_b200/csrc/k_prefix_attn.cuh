@@ -632,21 +632,31 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     prefetch_tmap(&kmap);
     prefetch_tmap(&vmap);
   }
-  griddep_wait();
-  griddep_launch();   // the row kernel may start now: what came before is done
+  // The kernel after this one may start once what came before both is done (griddep_launch follows the
+  // wait).  After the shared prefix's kernel, of which nothing is read here, this one takes the SMs that
+  // it leaves free, and ends after it.
+  const bool beside = OWN && p.own_only;
+  if (!beside) griddep_wait();
+  griddep_launch();
 
   // ---- the rows and keys of this CTA (the same in every thread)
   int b = 0, ti = blockIdx.x;
   int tok0 = 0, n_rows, own = 0, first_lim = p.prefix_len, last_lim = p.prefix_len;
   if (OWN) {
-    if (!find_tile(p, blockIdx.x, 2 * kTile, lane, b, ti)) return;
+    if (!find_tile(p, blockIdx.x, 2 * kTile, lane, b, ti)) {
+      if (beside) griddep_wait();
+      return;
+    }
     tok0 = p.cu_q[b];
     const int nq = p.cu_q[b + 1] - tok0;
     const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
     own = max(0, min(given, cap));
     n_rows = min(2 * kTile, nq * p.group - ti * 2 * kTile);
     if ((given > cap || tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) && threadIdx.x == 0) ops::report(p.status, kDevBadIndex);
-    if (tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) return;
+    if (tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) {
+      if (beside) griddep_wait();
+      return;
+    }
     first_lim = p.prefix_len + own - nq + 1;
     last_lim = max(0, first_lim + (ti * 2 * kTile + n_rows - 1) / p.group);
   } else {
@@ -947,6 +957,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 512);
   }
+  if (beside) griddep_wait();
 }
 
 // ---------------------------------------------------------------- joining key ranges

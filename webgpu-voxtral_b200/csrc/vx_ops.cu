@@ -130,14 +130,15 @@ struct Plan {
   int64_t bytes;
 };
 
-// Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's
-// share of the key tiles least, a range's start and end (loading Q,
-// writing the partial) counted as four tiles.
-int tile_parts(long long items, long long tiles, int sms) {
+// Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's share of the
+// key tiles least.  A range's start and end (loading Q, writing the partial) count as four tiles
+// (a tile of 2 x 128 rows takes 2.2 us), and each range's partial is written and read once more.
+int tile_parts(long long items, long long tiles, double partial_bytes, int sms) {
+  const double join = 2.0 * partial_bytes / 6e6 / 2.2;
   int best = 1;
   double least = 1e300;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 4.0);
+    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 4.0) + s * join;
     if (cost < least * 0.999) {
       least = cost;
       best = s;
@@ -176,17 +177,18 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   // Where that would take longer than the tile kernel's start and end, the rows of all sequences
   // take the prefix together; not where the sequences' rows fill tiles by themselves, and partials of
   // the prefix and of the own keys would only add to the work.
+  const double partial = (double)a.n_tokens * a.n_heads * c.head_dim * 4;
   const double again = (double)(a.cu_q ? rows / 32 + a.n_seqs : a.n_seqs) * a.prefix_len * c.n_kv_heads * c.head_dim * 4;
   if (a.n_seqs > 1 && again > kSharePrefixBytes && each < 512) {
     pl.shared_pairs = (rows + 255) / 256;
-    pl.shared_parts = tile_parts(pl.shared_pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, sms);
+    pl.shared_parts = tile_parts(pl.shared_pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, partial, sms);
   }
-  // The tile kernel multiplies 128 rows at once; of sequences with fewer than 64 (256 for the own keys
-  // alone, of which there are fewer) the row kernel's tiles of 32 waste less
-  if (a.cu_q && own_keys + a.prefix_len && each >= (pl.shared_pairs ? 256 : 64)) {
+  // The tile kernel multiplies 128 rows at once; of sequences with fewer than 64 the row kernel's tiles of
+  // 32 waste less
+  if (a.cu_q && own_keys + a.prefix_len && each >= 64) {
     pl.own_pairs = rows / 256 + a.n_seqs;
     const long long keys = (pl.shared_pairs ? 0 : (a.prefix_len + 127) / 128) + (own_keys + 127) / 128;
-    pl.own_parts = keys ? tile_parts(pl.own_pairs * c.n_kv_heads, keys, sms) : 0;
+    pl.own_parts = keys ? tile_parts(pl.own_pairs * c.n_kv_heads, keys, partial, sms) : 0;
     if (!keys) pl.own_pairs = 0;
   } else if (own_keys || !pl.shared_pairs) {
     pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
