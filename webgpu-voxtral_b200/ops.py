@@ -28,6 +28,7 @@ import torch
 from .engine import VX_OK, VoxtralError, load_library
 
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_HALF = (torch.float16, torch.bfloat16)
 _INT = torch.int32
 _CACHE = "2P6q6i"                                # vx_kv_pages
 _APPEND = struct.Struct("@" + _CACHE + "4P8q5Pq8i")   # vx_rope_append_args
@@ -55,9 +56,8 @@ def _library():
 
 def _call(fn, args: bytes, device: int):
     """fn on torch's current stream of the device, which is made current for the call."""
-    try:
-        err = _local.err
-    except AttributeError:
+    err = getattr(_local, "err", None)
+    if err is None:
         err = _local.err = ctypes.create_string_buffer(_ERR)
     if device == torch.cuda.current_device():
         rc = fn(args, torch._C._cuda_getCurrentRawStream(device), err, _ERR)
@@ -68,27 +68,27 @@ def _call(fn, args: bytes, device: int):
         raise VoxtralError(rc, err.value.decode())
 
 
-def _same_place(names: str, *tensors):
-    """The device that holds them all."""
-    device = tensors[0].get_device()
-    for i, t in enumerate(tensors):
+def _misplaced(names: str, *tensors):
+    """Says which of the tensors is not where the first one is."""
+    device, first = tensors[0].get_device(), names.split()[0]
+    for name, t in zip(names.split(), tensors):
         if t is not None and (t.get_device() != device or device < 0):
-            first, name = names.split()[0], names.split()[i]
             _refuse(f"{name} must be on a CUDA device, not {t.device}" if device < 0 else f"{name} is on {t.device}, {first} on cuda:{device}")
-    return device
+    _refuse("tensors must be on one CUDA device")
 
 
-def _rows(name, t, dims, *dtypes):
+def _rows(name, t, dims, dtypes):
     """Shape and strides of a tensor of rows."""
     shape, stride = t.shape, t.stride()
-    if len(shape) != dims:
-        _refuse(f"{name} must have {dims} dimensions, not {len(shape)}")
-    if t.dtype not in dtypes:
-        _refuse(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, not {t.dtype}")
-    if stride[-1] != 1 and shape[-1] > 1:
-        _refuse(f"{name}: the last dimension must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(f"{name} requires a gradient, which this operator does not compute")
+    if len(shape) != dims or t.dtype not in dtypes or stride[-1] != 1 or t.requires_grad:
+        if len(shape) != dims:
+            _refuse(f"{name} must have {dims} dimensions, not {len(shape)}")
+        if t.dtype not in dtypes:
+            _refuse(f"{name} must be one of {', '.join(str(d) for d in dtypes)}, not {t.dtype}")
+        if stride[-1] != 1 and shape[-1] > 1:
+            _refuse(f"{name}: the last dimension must be contiguous")
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name} requires a gradient, which this operator does not compute")
     return shape, stride
 
 
@@ -101,8 +101,8 @@ def _vector(name, t, dtype, n=None):
 
 
 def _cache(k_pages, v_pages):
-    shape, ks = _rows("k_pages", k_pages, 4, torch.float16, torch.bfloat16)
-    shape_v, vs = _rows("v_pages", v_pages, 4, k_pages.dtype)
+    shape, ks = _rows("k_pages", k_pages, 4, _HALF)
+    shape_v, vs = _rows("v_pages", v_pages, 4, (k_pages.dtype,))
     if shape != shape_v:
         _refuse(f"k_pages {tuple(shape)} and v_pages {tuple(shape_v)} must have one shape")
     return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], *shape, _DTYPE[k_pages.dtype], 0)
@@ -133,8 +133,8 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     padding, of which nothing is written).  rope_freq: f32 [rot_dim / 2], the angle of pair i at
     position p is p * rope_freq[i]; pairs are neighbours (interleaved) or the two halves.
     Returns the rotated q in the cache's type (q_out, if given; it may be q itself)."""
-    shape, ks = _rows("k", k, 3, *_DTYPE)
-    shape_v, vs = _rows("v", v, 3, k.dtype)
+    shape, ks = _rows("k", k, 3, _DTYPE)
+    shape_v, vs = _rows("v", v, 3, (k.dtype,))
     cache = _cache(k_pages, v_pages)
     n, kv, d = shape
     if shape_v != shape or kv != cache[9] or d != cache[11]:
@@ -146,19 +146,23 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     heads = q_ptr = out_ptr = 0
     qs = os = (0, 0)
     if q is not None:
-        shape_q, qs = _rows("q", q, 3, k.dtype)
+        shape_q, qs = _rows("q", q, 3, (k.dtype,))
         if shape_q[0] != n or shape_q[2] != d:
             _refuse(f"q {tuple(shape_q)} does not fit k {tuple(shape)}")
         if q_out is None:
             q_out = k_pages.new_empty(shape_q)
-        shape_o, os = _rows("q_out", q_out, 3, k_pages.dtype)
+        shape_o, os = _rows("q_out", q_out, 3, (k_pages.dtype,))
         if shape_o != shape_q:
             _refuse(f"q_out {tuple(shape_o)} must have q's shape {tuple(shape_q)}")
         heads, q_ptr, out_ptr = shape_q[1], q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _refuse("q_out without q")
-    device = _same_place("k q v k_pages v_pages page_table seq_ids positions rope_freq q_out status", k, q, v, k_pages, v_pages,
-                         page_table, seq_ids, positions, rope_freq, q_out, status)
+    device = k.get_device()
+    if not (0 <= device == v.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device()
+            == seq_ids.get_device() == positions.get_device() == rope_freq.get_device()
+            and (q is None or q.get_device() == device == q_out.get_device()) and (status is None or status.get_device() == device)):
+        _misplaced("k q v k_pages v_pages page_table seq_ids positions rope_freq q_out status", k, q, v, k_pages, v_pages,
+                   page_table, seq_ids, positions, rope_freq, q_out, status)
     _call(_library().vx_rope_append_kv,
           _APPEND.pack(*cache, q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
                        page_table.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), rope_freq.data_ptr(), _status(status), table_stride,
@@ -205,10 +209,10 @@ def shared_prefix_attention_workspace(q, k_pages, v_pages, prefix_pages, prefix_
 def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status):
     """(cache, sizes, pointers and strides from q to status and then the table's stride, device)"""
     cache = _cache(k_pages, v_pages)
-    shape, qs = _rows("q", q, 3, k_pages.dtype)
+    shape, qs = _rows("q", q, 3, (k_pages.dtype,))
     if shape[2] != cache[11]:
         _refuse(f"q {tuple(shape)} does not fit a cache with head_dim {cache[11]}")
-    shape_o, os = _rows("out", out, 3, k_pages.dtype)
+    shape_o, os = _rows("out", out, 3, (k_pages.dtype,))
     if shape_o != shape:
         _refuse(f"out {tuple(shape_o)} must have q's shape {tuple(shape)}")
     seqs, pages, table_stride = _table(page_table)
@@ -218,8 +222,12 @@ def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suff
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_pages.shape[0]} pages of {cache[10]}")
     if cu_q is not None:
         _vector("cu_q", cu_q, _INT, seqs + 1)
-    device = _same_place("q k_pages v_pages prefix_pages page_table suffix_lens cu_q out status", q, k_pages, v_pages, prefix_pages,
-                         page_table, suffix_lens, cu_q, out, status)
+    device = q.get_device()
+    if not (0 <= device == k_pages.get_device() == v_pages.get_device() == prefix_pages.get_device() == page_table.get_device()
+            == suffix_lens.get_device() == out.get_device() and (cu_q is None or cu_q.get_device() == device)
+            and (status is None or status.get_device() == device)):
+        _misplaced("q k_pages v_pages prefix_pages page_table suffix_lens cu_q out status", q, k_pages, v_pages, prefix_pages,
+                   page_table, suffix_lens, cu_q, out, status)
     sizes = (*cache[8:13], cu_q is not None, shape[0], seqs, shape[1], prefix_len, pages)
     pointers = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], prefix_pages.data_ptr(), page_table.data_ptr(),
                 suffix_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), _status(status), table_stride)
@@ -244,22 +252,20 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     running mass reaches u times the kept mass.  temperature 0 takes the first.  Each setting is a
     tensor by row (f32; top_k int32), or a number, which counts as such a tensor of that value.  Returns int32 [n_rows]; -1 for a row whose
     logits are all -inf or NaN."""
-    shape, stride = _rows("logits", logits, 2, *_DTYPE)
+    shape, stride = _rows("logits", logits, 2, _DTYPE)
     rows, cols = shape
     if u.dtype is not torch.float64 or u.shape != (rows,) or not u.is_contiguous():
         _refuse(f"u must be a contiguous float64 tensor of {rows} elements, not {u.dtype} {tuple(u.shape)}")
-    tensors, each, one = [logits, u], [], []
-    for name, v, kind in (("temperature", temperature, torch.float32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32),
-                          ("top_k", top_k, _INT)):
+    tensors, each, one = [logits, u], [0, 0, 0, 0], [temperature, top_p, min_p, top_k]
+    for i in range(4):
+        v = one[i]
         if isinstance(v, torch.Tensor):
+            kind = torch.float32 if i < 3 else _INT
             if v.dtype is not kind or v.shape != (rows,) or not v.is_contiguous():
-                _refuse(f"{name} must be a number or a contiguous {kind} tensor of {rows} elements, not {v.dtype} {tuple(v.shape)}")
+                _refuse(f"{('temperature', 'top_p', 'min_p', 'top_k')[i]} must be a number or a contiguous {kind} tensor of {rows} elements, "
+                        f"not {v.dtype} {tuple(v.shape)}")
             tensors.append(v)
-            each.append(v.data_ptr())
-            one.append(0)
-        else:
-            each.append(0)
-            one.append(v)
+            each[i], one[i] = v.data_ptr(), 0
     if not -2**31 <= one[3] < 2**31:
         _refuse(f"top_k {one[3]} does not fit 32 bits")
     if out is None:
@@ -267,7 +273,9 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     else:
         _vector("out", out, _INT, rows)
         tensors.append(out)
-    device = _same_place("logits u setting setting setting setting out", *tensors)
+    device = logits.get_device()
+    if device < 0 or any(t.get_device() != device for t in tensors):
+        _misplaced("logits u setting setting setting setting out", *tensors)
     _call(_library().vx_sample_logits,
           _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), stride[0], one[0], one[1], one[2], int(one[3]),
                        _DTYPE[logits.dtype], rows, cols, 0), device)
