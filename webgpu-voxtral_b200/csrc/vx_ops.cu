@@ -132,13 +132,17 @@ struct Plan {
 
 // Key ranges of the tile kernel: one CTA an SM, so the number that makes the slowest SM's share of the
 // key tiles least.  A range's start and end (loading Q, writing the partial) count as four tiles
-// (a tile of 2 x 128 rows takes 2.2 us), and each range's partial is written and read once more.
-int tile_parts(long long items, long long tiles, double partial_bytes, int sms) {
-  const double join = 2.0 * partial_bytes / 6e6 / 2.2;
+// (a tile of 2 x 128 rows takes 2.2 us), and each range's partial is written and read once more.  Where
+// the row kernel runs beside it for `row_us`, the fewest ranges that take half as long leave it the most SMs:
+// 64 sequences past 617 shared keys with 1, 2, 3, 5 ranges 27, 25, 27, 31 us in all.
+int tile_parts(long long items, long long tiles, double partial_bytes, double row_us, int sms) {
+  constexpr double kTileUs = 2.2;
+  const double join = 2.0 * partial_bytes / 6e6 / kTileUs;
   int best = 1;
   double least = 1e300;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {
     const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 4.0) + s * join;
+    if (cost * kTileUs <= row_us / 2) return s;
     if (cost < least * 0.999) {
       least = cost;
       best = s;
@@ -179,16 +183,18 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   // the prefix and of the own keys would only add to the work.
   const double partial = (double)a.n_tokens * a.n_heads * c.head_dim * 4;
   const double again = (double)(a.cu_q ? rows / 32 + a.n_seqs : a.n_seqs) * a.prefix_len * c.n_kv_heads * c.head_dim * 4;
+  // the row kernel beside it: its own start and end, and half the keys that the page tables can hold
+  const double row_us = a.cu_q ? 0.0 : 8.0 + (double)a.n_seqs * own_keys * c.n_kv_heads * c.head_dim * 2 / 6.4e6;
   if (a.n_seqs > 1 && again > kSharePrefixBytes && each < 512) {
     pl.shared_pairs = (rows + 255) / 256;
-    pl.shared_parts = tile_parts(pl.shared_pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, partial, sms);
+    pl.shared_parts = tile_parts(pl.shared_pairs * c.n_kv_heads, (a.prefix_len + 127) / 128, partial, row_us, sms);
   }
   // The tile kernel multiplies 128 rows at once; of sequences with fewer than 64 the row kernel's tiles of
   // 32 waste less
   if (a.cu_q && own_keys + a.prefix_len && each >= 64) {
     pl.own_pairs = rows / 256 + a.n_seqs;
     const long long keys = (pl.shared_pairs ? 0 : (a.prefix_len + 127) / 128) + (own_keys + 127) / 128;
-    pl.own_parts = keys ? tile_parts(pl.own_pairs * c.n_kv_heads, keys, partial, sms) : 0;
+    pl.own_parts = keys ? tile_parts(pl.own_pairs * c.n_kv_heads, keys, partial, 0.0, sms) : 0;
     if (!keys) pl.own_pairs = 0;
   } else if (own_keys || !pl.shared_pairs) {
     pl.nt = a.cu_q || group > 16 ? 4 : group > 8 ? 2 : 1;
@@ -403,10 +409,11 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   const int sms = sm_count();
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
   // CTAs a row: more of them while all rows together give an SM less than one and a half (two fit),
-  // none with fewer than 8192 logits.  One B200: 64 rows of 131072 bf16 logits with 2, 4, 8 CTAs a row
-  // 47, 35, 43 us; 200 rows of f32 with 1, 2, 4 158, 143, 162 us; one row with 1, 4, 8 95, 36, 26 us
+  // none with fewer than 16384 logits.  One B200: 64 rows of 131072 bf16 logits with 2, 4, 8 CTAs a row
+  // 47, 35, 43 us; 200 rows of f32 with 1, 2, 4 158, 143, 162 us; one row with 1, 4, 8 95, 36, 26 us; 64
+  // rows of 8320 with 1, 2 CTAs 10, 12 us
   int cluster = 1;
-  while (cluster < sample::kMaxCluster && 2ll * a.n_rows * cluster < 3ll * sms && a.n_cols > 8192 * cluster) cluster *= 2;
+  while (cluster < sample::kMaxCluster && 2ll * a.n_rows * cluster < 3ll * sms && a.n_cols > 16384 * cluster) cluster *= 2;
   if ((long long)a.n_rows * cluster > 0x7fffffff) return e.fail(VX_E_RANGE, "%d rows are too many for one call", a.n_rows);
   sample::Params p{};
   p.logits = a.logits; p.stride = a.row_stride; p.u = a.u;
