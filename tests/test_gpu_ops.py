@@ -540,3 +540,65 @@ def test_operators_on_several_streams(vx):
         torch.cuda.synchronize()
         for x, r in zip(steps, res):
             x.check(*r)
+
+
+def test_operators_captured_as_their_first_call(vx):
+    """In a fresh process nothing has been set up yet when the capture begins."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import importlib, torch
+vx = importlib.import_module("webgpu-voxtral_b200")
+c = dict(device="cuda")
+kp, vp = torch.zeros(90, 8, 64, 128, dtype=torch.float16, **c), torch.randn(90, 8, 64, 128, **c).half()
+q, k = torch.randn(64, 32, 128, **c).half(), torch.randn(64, 8, 128, **c).half()
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, **c)
+pp, table, pos, seq = i32(list(range(20))), i32([[20 + b] for b in range(64)]), i32([0] * 64), i32(list(range(64)))
+fr, u = torch.ones(64, **c), torch.full((64,), 0.5, dtype=torch.float64, **c)
+w = torch.randn(4096, 40000, **c).half()
+def step():
+    r = vx.rope_append_kv(q, k, k, kp, vp, table, seq, pos, fr)
+    o = vx.shared_prefix_attention(r, kp, vp, pp, 1280, table, pos + 1)
+    x = vx.shared_prefix_attention(r, kp, vp, pp, 1280, table, pos + 1, cu_q=i64)
+    return r, o, x, vx.sample_logits(o.flatten(1) @ w, u, top_p=0.9)
+i64 = i32(list(range(65)))
+torch.zeros(1, **c) @ torch.zeros(1, **c)
+g = torch.cuda.CUDAGraph()
+s = torch.cuda.Stream()
+with torch.cuda.stream(s):
+    torch.zeros(64, 4096, **c).half() @ w       # the library's own workspace
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=s):
+    a = step()
+g.replay()
+torch.cuda.synchronize()
+b = step()
+assert all(torch.equal(x, y) for x, y in zip(a[:2], b[:2])) and (a[1].float() - a[2].float()).abs().max() < 2e-2
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(vx.library_path()))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_attend_without_own_pages(vx):
+    """A page table of no columns: the prefix alone, through each kernel that may take it."""
+    for seqs, prefix in ((2, 100), (64, 2000)):
+        q, kp, vp, ppages, table, suffix, cu = attend_inputs([(1, 0)] * seqs, prefix, 32, 8, 128, 64, F16, False, seed=seqs)
+        want, tol = attend_reference(q[:seqs], kp, vp, ppages, prefix, table, [(1, 0)] * seqs, 128 ** -0.5)
+        for kw in ({}, {"cu_q": cu}):
+            got = vx.shared_prefix_attention(q[:seqs], kp, vp, ppages, prefix, table[:, :0], suffix, **kw)
+            assert torch.all((got.double() - want).abs() <= tol)
+
+
+def test_attend_workspace(vx):
+    q, kp, vp, ppages, table, suffix, _ = attend_inputs([(1, 30), (1, 3)], 500, 8, 2, 64, 16, F16, False, seed=6)
+    need = vx.shared_prefix_attention_workspace(q[:2], kp, vp, ppages, 500, table, suffix)
+    want = vx.shared_prefix_attention(q[:2], kp, vp, ppages, 500, table, suffix)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")               # NaN in every float
+    assert torch.equal(want, vx.shared_prefix_attention(q[:2], kp, vp, ppages, 500, table, suffix, workspace=ws))
+    with pytest.raises(vx.VoxtralError, match="workspace"):
+        vx.shared_prefix_attention(q[:2], kp, vp, ppages, 500, table, suffix, workspace=ws[:need - 1])
+    with pytest.raises(vx.VoxtralError, match="workspace"):
+        vx.shared_prefix_attention(q[:2], kp, vp, ppages, 500, table, suffix, workspace=torch.empty(need + 64, dtype=torch.uint8, device="cuda")[1:])
