@@ -357,10 +357,11 @@ int vx_lm_head_argmax_noalloc(const uint16_t* weight, const float* x, int32_t ro
  * with an f32 cache (src/engine.ts:814-1042).
  * Element types: 0 F16, 1 BF16, 2 F32 (as in vx_load_tensor_typed).  Strides count elements; the
  * innermost dimension is contiguous; rows start on 16-byte boundaries.
- * status (nullable, int32, set to 0 by the caller): keeps the first VX_STATUS_* a kernel met. */
-#define VX_STATUS_WAIT_1 1    /* a bounded wait of a kernel expired (codes 1 to 4 and 6)       */
+ * status (nullable, int32, set to 0 by the caller): the first thing that went wrong on the device, 0 if
+ * nothing did: VX_STATUS_BAD_INDEX, or another code where a bounded wait of a kernel expired (the
+ * output is then not valid). */
 #define VX_STATUS_BAD_INDEX 5 /* a page, sequence, offset or length out of range: such a token is
-                                 not written, keys of such a page read as zero                 */
+                                 not written, keys of such a page read as zero */
 
 /* One layer of a paged K/V cache: element (page, head, slot, d) of each pool at
  * page * page_stride + head * head_stride + slot * slot_stride + d.  The engine's own layout
@@ -376,8 +377,9 @@ typedef struct vx_kv_pages {
 /* Rotary positions and the cache append of a ragged batch.  Token t of sequence seq_ids[t] at
  * position positions[t]: q (n_heads rows; n_heads 0: none) rotated into q_out in the cache's type,
  * k rotated and v unchanged written to slot position % page_size of page
- * page_table[seq * table_stride + position / page_size].  Pair i turns by position * rope_freq[i]
- * (formed in f64): elements (2i, 2i+1) if interleaved, else (i, i + rot_dim / 2); elements from
+ * page_table[seq * table_stride + position / page_size].  Pair i turns by r * rope_freq[i] (formed in
+ * f64), r = rope_positions[t], or positions[t] where rope_positions is null (they differ where the
+ * page table begins after a shared prefix): elements (2i, 2i+1) if interleaved, else (i, i + rot_dim / 2); elements from
  * rot_dim on pass through.  A negative position is padding: nothing of that token is written.
  * Two tokens for one slot leave either (or a mixture).  q_out may be q itself where the
  * types are the same.  head_dim and rot_dim: multiples of 16, at most 512. */
@@ -387,7 +389,7 @@ typedef struct vx_rope_append_args {
   void* q_out;
   int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
   int64_t q_out_token_stride, q_out_head_stride;
-  const int32_t *page_table, *seq_ids, *positions;
+  const int32_t *page_table, *seq_ids, *positions, *rope_positions;
   const float* rope_freq; /* [rot_dim / 2] */
   int32_t* status;
   int64_t table_stride;
@@ -402,6 +404,7 @@ int vx_rope_append_kv(const vx_rope_append_args* a, void* stream, char* err, siz
  * query token stands at the last key, the others before it, and each sees the keys up to its own
  * position (the keys of the query tokens must be in the cache already); a token that sees no
  * key gives 0.  out = softmax(q k * scale) v, rows as q; rows of no sequence are not written.
+ * A negative length counts as 0.  out must not overlap q or the cache.
  * n_heads a multiple of the cache's n_kv_heads; head_dim 64 or 128; page_size 16, 32, 64, 128 or
  * 256; q and out in the cache's type; scale > 0.  Keys that no query token sees may hold any
  * value (NaN too) where they lie past the prefix or past a sequence's keys; keys that some token

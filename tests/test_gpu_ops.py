@@ -120,6 +120,16 @@ def test_append(vx, io, cache, inter, heads, kv, dim, rot, page, tm, lens, start
     assert torch.all(kp == 7.0) and torch.all(vp == 7.0)                     # nothing else is written
 
 
+def test_append_rotates_by_other_positions(vx):
+    kp, vp = pool(2, 2, 16, 64, BF16, fill=7.0), pool(2, 2, 16, 64, BF16, fill=7.0)
+    q, k, v = rand(3, 4, 64, dtype=BF16, seed=1), rand(3, 2, 64, dtype=BF16, seed=2), rand(3, 2, 64, dtype=BF16, seed=3)
+    turn = ints([700, -5, 10_000_000])
+    out = vx.rope_append_kv(q, k, v, kp, vp, ints([[1]]), ints([0, 0, 0]), ints([0, 15, 7]), freqs(64), rope_positions=turn)
+    for x, got in ((q, out), (k, kp[1][:, [0, 15, 7]].transpose(0, 1))):
+        y, mag = rotated(x, turn, freqs(64), True)
+        check_rounded(got, y, mag)
+
+
 def test_append_in_place_and_bad_indices(vx):
     kp, vp = pool(3, 2, 16, 64, F16, fill=7.0), pool(3, 2, 16, 64, F16, fill=7.0)
     q, k, v = rand(5, 4, 64, dtype=F16, seed=1), rand(5, 2, 64, dtype=F16, seed=2), rand(5, 2, 64, dtype=F16, seed=3)
@@ -482,7 +492,8 @@ class Step:
     def run(self):
         h, kv = self.heads, self.kv
         q, k, v = self.qkv[:, :h], self.qkv[:, h:h + kv], self.qkv[:, h + kv:]
-        q = self.vx.rope_append_kv(q, k, v, self.kp, self.vp, self.table, self.seq, self.pos, self.freq)
+        q = self.vx.rope_append_kv(q, k, v, self.kp, self.vp, self.table, self.seq, self.pos, self.freq,
+                                   rope_positions=self.pos + self.prefix)
         o = self.vx.shared_prefix_attention(q, self.kp, self.vp, self.ppages, self.prefix, self.table, self.lens)
         logits = o.flatten(1) @ self.w
         return q, o, logits, self.vx.sample_logits(logits, self.u, temperature=0.9, top_k=300, top_p=0.97)

@@ -50,6 +50,7 @@ def _append(**kw):
     (dict(k_pages=torch.zeros(5, 3, 16, 64, dtype=F16), v_pages=torch.zeros(5, 3, 16, 64, dtype=F16)), "do not fit a cache"),
     (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions must be"),
     (dict(seq_ids=ints([0, 0])), "seq_ids must have 3"),
+    (dict(rope_positions=ints([0, 0])), "rope_positions must have 3"),
     (dict(page_table=ints([0, 1])), "page_table must be"),
     (dict(q_out=torch.zeros(3, 4, 64, dtype=BF16)), "q_out must be one of"),
     (dict(k=torch.zeros(3, 64, 2, dtype=F16).transpose(1, 2)), "last dimension"),
@@ -138,7 +139,7 @@ def _cache(**kw):
     ({}, dict(n_tokens=0), 0, ""),
 ])
 def test_append_c_refuses(ops, cache, change, code, word):
-    a = dict(q=P, k=P, v=P, q_out=P, qs=256, qh=64, kst=128, kh=64, vst=128, vh=64, os=256, oh=64, table=P, seq=P, pos=P, freq=P, status=0,
+    a = dict(q=P, k=P, v=P, q_out=P, qs=256, qh=64, kst=128, kh=64, vst=128, vh=64, os=256, oh=64, table=P, seq=P, pos=P, rpos=0, freq=P, status=0,
              tstride=4, dtype=0, n_tokens=3, heads=4, n_seqs=1, max_pages=2, rot=64, inter=1, reserved=0)
     a.update(change)
     rc, msg = _c(ops, "vx_rope_append_kv", ops._APPEND.pack(*_cache(**cache), *a.values()))

@@ -1,10 +1,10 @@
 // k_rope_append.cuh — rotary positions on q and k, and k / v appended to a paged cache.
 //
-// For a token at position p, with frequency f_i of pair i:
+// For a token at (rotary) position p, with frequency f_i of pair i:
 //   (a, b) -> (a cos(p f_i) - b sin(p f_i), a sin(p f_i) + b cos(p f_i)),
 // pairs (2i, 2i+1) (interleaved) or (i, i + rot/2); values past rot_dim pass through.
-// q goes to q_out in the cache's type, k and v to slot p % page_size of the page that
-// page_table[seq][p / page_size] names.
+// q goes to q_out in the cache's type, k and v to slot c % page_size of the page that
+// page_table[seq][c / page_size] names, c the position in the cache (p itself unless given apart).
 //
 // The angle is reduced in 64 bits: p f_i / 2 pi as a double, its nearest whole number taken
 // off, and only the remainder (under half a turn) rounded to f32 for sincospif.  In f32 the
@@ -26,7 +26,7 @@ struct Params {
   void *q_out, *k_pages, *v_pages;
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head;      // element strides
   long long kp_page, kp_head, kp_slot, vp_page, vp_head, vp_slot;
-  const int32_t *page_table, *seq_ids, *positions;
+  const int32_t *page_table, *seq_ids, *positions, *rope_positions;
   const float* freq;
   int32_t* status;
   long long table_stride;
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) k_rope_append(const __grid_constant__ Par
   griddep_launch();
   griddep_wait();
   const int t = blockIdx.x;
-  const int pos = p.positions[t], seq = p.seq_ids[t];
+  const int pos = p.positions[t], seq = p.seq_ids[t], turn_pos = p.rope_positions ? p.rope_positions[t] : pos;
   if (pos < 0) return;   // padding
   const int lp = pos / p.page_size, slot = pos % p.page_size;
   const bool in_table = seq >= 0 && seq < p.n_seqs && lp < p.max_pages;
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) k_rope_append(const __grid_constant__ Par
     return;
   }
   for (int i = threadIdx.x; i < p.rot_dim / 2; i += blockDim.x) {
-    const double turns = (double)pos * (double)p.freq[i] * 0.15915494309189533577;   // / (2 pi)
+    const double turns = (double)turn_pos * (double)p.freq[i] * 0.15915494309189533577;   // / (2 pi)
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = c;

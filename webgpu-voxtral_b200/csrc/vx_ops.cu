@@ -323,7 +323,7 @@ extern "C" int vx_rope_append_kv(const vx_rope_append_args* ap, void* stream, ch
   p.v_tok = a.v_token_stride; p.v_head = a.v_head_stride; p.qo_tok = a.q_out_token_stride; p.qo_head = a.q_out_head_stride;
   p.kp_page = c.k_page_stride; p.kp_head = c.k_head_stride; p.kp_slot = c.k_slot_stride;
   p.vp_page = c.v_page_stride; p.vp_head = c.v_head_stride; p.vp_slot = c.v_slot_stride;
-  p.page_table = a.page_table; p.seq_ids = a.seq_ids; p.positions = a.positions; p.freq = a.rope_freq; p.status = a.status;
+  p.page_table = a.page_table; p.seq_ids = a.seq_ids; p.positions = a.positions; p.rope_positions = a.rope_positions; p.freq = a.rope_freq; p.status = a.status;
   p.table_stride = a.table_stride; p.n_tokens = a.n_tokens; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads;
   p.head_dim = c.head_dim; p.rot_dim = a.rot_dim; p.page_size = c.page_size; p.n_pages = c.n_pages; p.n_seqs = a.n_seqs;
   p.max_pages = a.max_pages;

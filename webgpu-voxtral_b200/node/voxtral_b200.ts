@@ -35,7 +35,7 @@ const vx_kv_pages = koffi.struct('vx_kv_pages', {
 koffi.struct('vx_rope_append_args', {
   cache: vx_kv_pages, q: 'void *', k: 'void *', v: 'void *', q_out: 'void *', q_token_stride: 'int64', q_head_stride: 'int64',
   k_token_stride: 'int64', k_head_stride: 'int64', v_token_stride: 'int64', v_head_stride: 'int64',
-  q_out_token_stride: 'int64', q_out_head_stride: 'int64', page_table: 'void *', seq_ids: 'void *', positions: 'void *',
+  q_out_token_stride: 'int64', q_out_head_stride: 'int64', page_table: 'void *', seq_ids: 'void *', positions: 'void *', rope_positions: 'void *',
   rope_freq: 'void *', status: 'void *', table_stride: 'int64', dtype: 'int32', n_tokens: 'int32', n_heads: 'int32',
   n_seqs: 'int32', max_pages: 'int32', rot_dim: 'int32', interleaved: 'int32', reserved: 'int32',
 });

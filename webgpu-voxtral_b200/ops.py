@@ -1,6 +1,7 @@
 """Serving operators on the caller's torch tensors: one step of a batch over a paged K/V cache.
 
-    q = rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, rope_freq)
+    q = rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, own_positions, rope_freq,
+                       rope_positions=own_positions + prefix_len)
     o = shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens)
     t = sample_logits(logits, u, temperature=0.8, top_k=50, top_p=0.95, min_p=0.02)
 
@@ -31,7 +32,7 @@ _DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _HALF = (torch.float16, torch.bfloat16)
 _INT = torch.int32
 _CACHE = "2P6q6i"                                # vx_kv_pages
-_APPEND = struct.Struct("@" + _CACHE + "4P8q5Pq8i")   # vx_rope_append_args
+_APPEND = struct.Struct("@" + _CACHE + "4P8q6Pq8i")   # vx_rope_append_args
 _PREFIX = struct.Struct("@" + _CACHE + "2P4q6P2q5if")  # vx_shared_prefix_args
 _SAMPLE = struct.Struct("@7Pq3f5i")              # vx_sample_args
 _ERR = 256
@@ -125,13 +126,15 @@ def _status(status):
 
 
 def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, rope_freq, *, interleaved: bool = True,
-                   q_out=None, status=None):
+                   rope_positions=None, q_out=None, status=None):
     """Rotates q and k of a ragged batch of tokens and appends k and v to a paged cache.
 
     q [n_tokens, n_heads, head_dim] (or None), k and v [n_tokens, n_kv_heads, head_dim]: f16, bf16
     or f32, one type.  Token t of sequence seq_ids[t] goes to position positions[t] (int32; negative:
     padding, of which nothing is written).  rope_freq: f32 [rot_dim / 2], the angle of pair i at
     position p is p * rope_freq[i]; pairs are neighbours (interleaved) or the two halves.
+    rope_positions (int32): the positions to rotate by where they are not those in the cache, as with
+    page tables that begin after a shared prefix.
     Returns the rotated q in the cache's type (q_out, if given; it may be q itself)."""
     shape, ks = _rows("k", k, 3, _DTYPE)
     shape_v, vs = _rows("v", v, 3, (k.dtype,))
@@ -142,6 +145,8 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     seqs, pages, table_stride = _table(page_table)
     _vector("seq_ids", seq_ids, _INT, n)
     _vector("positions", positions, _INT, n)
+    if rope_positions is not None:
+        _vector("rope_positions", rope_positions, _INT, n)
     _vector("rope_freq", rope_freq, torch.float32)
     heads = q_ptr = out_ptr = 0
     qs = os = (0, 0)
@@ -160,12 +165,13 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     device = k.get_device()
     if not (0 <= device == v.get_device() == k_pages.get_device() == v_pages.get_device() == page_table.get_device()
             == seq_ids.get_device() == positions.get_device() == rope_freq.get_device()
-            and (q is None or q.get_device() == device == q_out.get_device()) and (status is None or status.get_device() == device)):
-        _misplaced("k q v k_pages v_pages page_table seq_ids positions rope_freq q_out status", k, q, v, k_pages, v_pages,
-                   page_table, seq_ids, positions, rope_freq, q_out, status)
+            and (q is None or q.get_device() == device == q_out.get_device()) and (status is None or status.get_device() == device)
+            and (rope_positions is None or rope_positions.get_device() == device)):
+        _misplaced("k q v k_pages v_pages page_table seq_ids positions rope_positions rope_freq q_out status", k, q, v, k_pages, v_pages,
+                   page_table, seq_ids, positions, rope_positions, rope_freq, q_out, status)
     _call(_library().vx_rope_append_kv,
           _APPEND.pack(*cache, q_ptr, k.data_ptr(), v.data_ptr(), out_ptr, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1],
-                       page_table.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), rope_freq.data_ptr(), _status(status), table_stride,
+                       page_table.data_ptr(), seq_ids.data_ptr(), positions.data_ptr(), 0 if rope_positions is None else rope_positions.data_ptr(), rope_freq.data_ptr(), _status(status), table_stride,
                        _DTYPE[k.dtype], n, heads, seqs, pages, 2 * rope_freq.shape[0], 1 if interleaved else 0, 0), device)
     return q_out
 
