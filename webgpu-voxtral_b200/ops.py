@@ -156,9 +156,11 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
             _refuse(f"q {tuple(shape_q)} does not fit k {tuple(shape)}")
         if q_out is None:
             q_out = k_pages.new_empty(shape_q)
-        shape_o, os = _rows("q_out", q_out, 3, (k_pages.dtype,))
-        if shape_o != shape_q:
-            _refuse(f"q_out {tuple(shape_o)} must have q's shape {tuple(shape_q)}")
+            os = q_out.stride()
+        else:
+            shape_o, os = _rows("q_out", q_out, 3, (k_pages.dtype,))
+            if shape_o != shape_q:
+                _refuse(f"q_out {tuple(shape_o)} must have q's shape {tuple(shape_q)}")
         heads, q_ptr, out_ptr = shape_q[1], q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _refuse("q_out without q")
@@ -187,9 +189,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     scale defaults to 1 / sqrt(head_dim).  Returns out, shaped as q; rows past cu_q's last are not
     written, a row that sees no key is 0.  workspace: a uint8 tensor of at least
     shared_prefix_attention_workspace bytes that no other call uses at the same time."""
-    if out is None:
-        out = q.new_empty(q.shape)
-    cache, sizes, pointers, device = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status)
+    cache, sizes, pointers, device, out = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status)
     need = _workspace_bytes(sizes, device)
     held = ptr = 0
     if workspace is not None:
@@ -197,7 +197,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
             _refuse(f"workspace must be a contiguous uint8 tensor on cuda:{device}")
         ptr, held = workspace.data_ptr(), workspace.numel()
     elif need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(need >> 1)       # 2-byte elements; need is a multiple of 4
         ptr, held = workspace.data_ptr(), need
     _call(_library().vx_shared_prefix_attention,
           _PREFIX.pack(*cache, *pointers[:11], ptr, held, pointers[11], *sizes[6:], 1.0 / math.sqrt(sizes[3]) if scale is None else scale),
@@ -208,19 +208,23 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
 def shared_prefix_attention_workspace(q, k_pages, v_pages, prefix_pages, prefix_len: int, page_table, suffix_lens, *, cu_q=None) -> int:
     """Bytes of workspace that shared_prefix_attention needs for these arguments.  They depend on
     shapes, prefix_len and whether cu_q is given, not on the values."""
-    _, sizes, _, device = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, q, None)
+    _, sizes, _, device, _ = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, q, None)
     return _workspace_bytes(sizes, device)
 
 
 def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status):
-    """(cache, sizes, pointers and strides from q to status and then the table's stride, device)"""
+    """(cache, sizes, pointers and strides from q to status and then the table's stride, device, out)"""
     cache = _cache(k_pages, v_pages)
     shape, qs = _rows("q", q, 3, (k_pages.dtype,))
     if shape[2] != cache[11]:
         _refuse(f"q {tuple(shape)} does not fit a cache with head_dim {cache[11]}")
-    shape_o, os = _rows("out", out, 3, (k_pages.dtype,))
-    if shape_o != shape:
-        _refuse(f"out {tuple(shape_o)} must have q's shape {tuple(shape)}")
+    if out is None:
+        out = q.new_empty(shape)
+        os = out.stride()
+    else:
+        shape_o, os = _rows("out", out, 3, (k_pages.dtype,))
+        if shape_o != shape:
+            _refuse(f"out {tuple(shape_o)} must have q's shape {tuple(shape)}")
     seqs, pages, table_stride = _table(page_table)
     _vector("suffix_lens", suffix_lens, _INT, seqs)
     _vector("prefix_pages", prefix_pages, _INT)
@@ -237,7 +241,7 @@ def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suff
     sizes = (*cache[8:13], cu_q is not None, shape[0], seqs, shape[1], prefix_len, pages)
     pointers = (q.data_ptr(), out.data_ptr(), qs[0], qs[1], os[0], os[1], prefix_pages.data_ptr(), page_table.data_ptr(),
                 suffix_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(), _status(status), table_stride)
-    return cache, sizes, pointers, device
+    return cache, sizes, pointers, device, out
 
 
 @functools.lru_cache(maxsize=1024)
