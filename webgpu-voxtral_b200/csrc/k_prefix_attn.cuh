@@ -969,9 +969,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
 
 // ---------------------------------------------------------------- joining key ranges
 // One warp per row (token, head): the maximum over its partials, then the weighted sums in the
-// order of the partials, so the result does not depend on timing.  Eight partials
-// are on their way at a time.
-template <typename T, int D>
+// order of the partials, so the result does not depend on timing.  U partials are on their way at
+// a time: with many rows four, for the fewer registers (62 against 96 at D 128) that let more
+// warps onto an SM (14000 rows of D 64 in a graph: 87.1 us for the whole call, with eight 91.8;
+// 20480 rows of D 128: 86.9 and 93.0), with few rows eight, for the latency of their many partials
+// (128 rows: 12.3 us, with four 13.4; 2048 rows: 25.4 and 26.1).
+template <typename T, int D, int U>
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Params p) {
   using E = ops::Elem<T>;
   constexpr int V = D / 32;   // values a lane
@@ -1010,10 +1013,10 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Param
       L += ml.y * f;
     }
     const int k = min(32, n - s0);
-    for (int s = 0; s < k; s += 8) {
-      float w[8], v[8][V];
+    for (int s = 0; s < k; s += U) {
+      float w[U], v[U][V];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < U; ++j) {
         w[j] = __shfl_sync(0xffffffffu, f, (s + j) & 31);
         if (s + j >= k) w[j] = 0.f;
 #pragma unroll
@@ -1030,7 +1033,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Param
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < U; ++j)
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] += v[j][i] * w[j];
     }

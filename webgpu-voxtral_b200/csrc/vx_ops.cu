@@ -274,7 +274,10 @@ cudaError_t launch_attention(const pattn::Params& p, const vx_kv_pages& c, const
          : pl.nt == 2 ? launch_rows<T, D, 2>(p, pl.row_ctas, s) : launch_rows<T, D, 4>(p, pl.row_ctas, s);
   if (ce != cudaSuccess || p.direct) return ce;
   const long long rows = (long long)p.n_tokens * p.n_heads;
-  return launch(pattn::k_attn_join<T, D>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
+  const dim3 grid((unsigned)((rows + 3) / 4));
+  // Above 8192 rows there are 55 warps an SM and more: occupancy counts, below it latency.
+  return rows >= 8192 ? launch(pattn::k_attn_join<T, D, 4>, grid, dim3(128), 0, s, p)
+                      : launch(pattn::k_attn_join<T, D, 8>, grid, dim3(128), 0, s, p);
 }
 
 // ------------------------------------------------------------------ sampling
