@@ -404,6 +404,8 @@ int vx_rope_append_kv(const vx_rope_append_args* a, void* stream, char* err, siz
  * query token stands at the last key, the others before it, and each sees the keys up to its own
  * position (the keys of the query tokens must be in the cache already); a token that sees no
  * key gives 0.  out = softmax(q k * scale) v, rows as q; rows of no sequence are not written.
+ * cu_q begins at 0 or later, never goes down and ends within n_tokens; the sequence whose beginning or end
+ * breaks that is refused with all after it (VX_STATUS_BAD_INDEX, their rows are not written).
  * A negative length counts as 0.  out must not overlap q or the cache.
  * n_heads a multiple of the cache's n_kv_heads; head_dim 64 or 128; page_size 16, 32, 64, 128 or
  * 256; q and out in the cache's type; scale > 0.  Keys that no query token sees may hold any

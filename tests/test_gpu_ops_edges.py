@@ -1,0 +1,61 @@
+"""The serving operators at the edges of what their documentation allows, and just past them: malformed
+offsets, lengths past a page table, settings at the ends of their range, page tables wider than needed.
+
+Tolerances and plain float64 forms are those of test_gpu_ops.py unless a test says otherwise."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_ops import BAD_INDEX, BF16, F16, attend_inputs, attend_reference, ints
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+MARGIN = 1 << 16
+
+
+def attend_in_margins(vx, *args, fill=0, **kw):
+    """shared_prefix_attention with a workspace of the least size between bytes that have to stay as they are."""
+    need = vx.shared_prefix_attention_workspace(*args, **{k: v for k, v in kw.items() if k == "cu_q"})
+    ws = torch.full((need + 2 * MARGIN,), 0xA5, dtype=torch.uint8, device="cuda")
+    ws[MARGIN:MARGIN + need] = fill
+    out = vx.shared_prefix_attention(*args, workspace=ws[MARGIN:MARGIN + need], **kw)
+    assert bool((ws[:MARGIN] == 0xA5).all()) and bool((ws[MARGIN + need:] == 0xA5).all())
+    return out
+
+
+OFFSETS = [  # (query tokens, own keys) of each sequence's cache, offsets, sequences in front of the bad one, prefix, dtype
+    ([(64, 70)] + [(0, 9)] * 63, [0, 64] * 32 + [0], 1, 0, F16),              # every second sequence decreases: by rows
+    ([(64, 70)] + [(0, 9)] * 63, [0, 64] * 32 + [0], 1, 2000, BF16),          # ... with the prefix by tiles
+    ([(100, 120), (0, 40), (0, 40), (100, 100)], [0, 100, 50, 200, 200], 1, 0, F16),    # whole sequences by tiles
+    ([(100, 120), (0, 40), (0, 40), (100, 100)], [0, 100, 50, 200, 200], 1, 700, BF16),
+    ([(3, 5), (4, 9), (0, 30)], [2, 5, 9, 4], 2, 40, F16),                    # the last one goes down
+    ([(3, 5), (4, 9), (0, 30)], [0, 3, 7, 900], 2, 40, F16),                  # past the batch
+    ([(3, 5), (4, 9), (0, 30)], [0, 3, 900, 7], 1, 40, BF16),
+    ([(3, 5), (4, 9), (2, 30)], [-1, 3, 6, 8], 0, 40, F16),                   # before it
+    ([(3, 5), (4, 9), (2, 30)], [-2**31, 2**31 - 1, 0, 3], 0, 40, F16),
+    ([(100, 0), (80, 0), (60, 0)], [0, 100, 180, 90], 2, 700, F16),           # the prefix alone
+]
+
+
+@pytest.mark.parametrize("case", range(len(OFFSETS)))
+def test_attend_offsets_out_of_order(vx, case):
+    """The sequences in front of the first bad offset are computed, the others refused; nothing is
+    written outside the workspace, nor into the refused ones' rows, whatever the workspace holds."""
+    lens, cu, held, prefix, dtype = OFFSETS[case]
+    q, kp, vp, ppages, table, suffix, _ = attend_inputs(lens, prefix, 32, 8, 128, 16, dtype, False, seed=case)
+    n = max([200 if len(lens) == 4 else 64 if len(lens) == 64 else 9] + cu[:held + 1])
+    first = max(cu[0], 0)
+    q = torch.cat((q, q[:1].expand(max(0, n + 2 - len(q)), -1, -1)))[:n + 2]
+    if not any(s for _, s in lens):
+        table = table[:, :0]
+    out, st = torch.full_like(q, 7.0), ints([0])
+    attend_in_margins(vx, q[:n], kp, vp, ppages, prefix, table, suffix, cu_q=ints(cu), out=out[:n], status=st)
+    assert int(st) == BAD_INDEX
+    want, tol = attend_reference(q[first:], kp, vp, ppages, prefix, table, lens[:held], 128 ** -0.5) if held else (q[:0], q[:0])
+    end = first + len(want)
+    assert end == (cu[held] if held else first)
+    off = (out[first:end].double() - want).abs() - tol
+    assert held == 0 or float(off.max()) <= 0
+    assert bool((out[:first] == 7.0).all()) and bool((out[end:] == 7.0).all())     # no sequence's rows, and refused ones'

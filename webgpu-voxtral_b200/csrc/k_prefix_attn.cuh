@@ -46,11 +46,11 @@ struct Params {
   float* row_o;              // partials of the row kernel: [part][8 NT][D]
   float2* row_ml;
   int2* row_parts;           // [n_tokens * n_heads]: first and last partial row; last -1: none, -2: out is written
+  int2* span;                // with cu_q and a join: the tokens [x, y) of the sequences that are held
   int n_tokens, n_seqs, n_heads, n_kv, group;
   int prefix_len, page_size, n_pages, max_pages;
   float scale_log2;          // scale * log2(e): weights are 2^(s * scale_log2 - m)
   int tile_parts;            // key ranges of the tile kernel (0: it does not run)
-  int row_rows;              // partial rows there is room for
   int rows_run;              // whether the row kernel runs, and the rows of its tiles
   int own_only;              // the prefix is the shared tile kernel's: the row kernel and the one of whole sequences leave it out
   int part0;                 // this tile launch's first partial
@@ -118,6 +118,37 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Offsets begin at 0 or later, never go down and end within the batch: sequences then share no row, and
+// have no more row tiles than the plan has room for.  The sequence whose beginning or end breaks that
+// is refused with all after it; those in front of it are held.
+__device__ __forceinline__ bool out_of_order(const Params& p, int b) {
+  const int from = p.cu_q[b], to = p.cu_q[b + 1];
+  return from < 0 || to < from || to > p.n_tokens;
+}
+// One thread says how many sequences are held: to the caller's status, and to the join.  (Every launch of
+// a call finds and writes the same.)
+__device__ __forceinline__ void tell_held(const Params& p, int n_seqs) {
+  if (n_seqs < p.n_seqs) ops::report(p.status, kDevBadIndex);
+  if (p.span) *p.span = make_int2(p.cu_q[0], p.cu_q[n_seqs]);
+}
+// Sequences that are held.  All threads of the block together: one pass over the offsets and, where they
+// are in order, one barrier.
+__device__ __forceinline__ int held_seqs(const Params& p) {
+  __shared__ int s_first;
+  if (!p.cu_q) return p.n_seqs;
+  int first = p.n_seqs;
+  for (int b = threadIdx.x; b < p.n_seqs && first == p.n_seqs; b += blockDim.x)
+    if (out_of_order(p, b)) first = b;
+  if (threadIdx.x == 0) s_first = p.n_seqs;
+  if (__syncthreads_or(first < p.n_seqs)) {
+    atomicMin(&s_first, first);
+    __syncthreads();
+    first = s_first;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) tell_held(p, first);
+  return first;
+}
+
 // ---------------------------------------------------------------- short row tiles
 // Up to 8 NT query rows of one sequence that share a K/V head are an item; its work is the 16-key
 // blocks of its sequence.  All blocks of all items stand in one line (sequence, row tile, head, block)
@@ -145,7 +176,7 @@ constexpr int row_smem() {
   return row_warps(D, NT) * row_warp_smem<D, NT>();
 }
 
-// A sequence as the row kernel sees it.
+// A sequence as the row kernel sees it (n_seqs: those of held_seqs).
 struct Seq {
   int tok0, nq, own, tiles, blocks;   // query tokens, own keys, row tiles, 16-key blocks (prefix and own)
   // An item counts kItemCost blocks more than it has: what its start (q, page numbers) and its end (a
@@ -153,18 +184,14 @@ struct Seq {
   __device__ __forceinline__ int item_units() const { return blocks ? blocks + kItemCost : 0; }
   __device__ __forceinline__ long long units(int n_kv) const { return (long long)tiles * n_kv * item_units(); }
 };
-__device__ __forceinline__ Seq sequence(const Params& p, int b, int rows) {
+__device__ __forceinline__ Seq sequence(const Params& p, int n_seqs, int b, int rows) {
   Seq q{0, 0, 0, 0, 0};
-  if (b >= p.n_seqs) return q;
+  if (b >= n_seqs) return q;
   q.tok0 = p.cu_q ? p.cu_q[b] : b;
   q.nq = p.cu_q ? p.cu_q[b + 1] - q.tok0 : 1;
   const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
   q.own = max(0, min(given, cap));
   if (given > cap) ops::report(p.status, kDevBadIndex);       // keys that the page table does not hold
-  if (q.tok0 < 0 || q.nq < 0 || q.tok0 + q.nq > p.n_tokens) {   // offsets that the batch does not hold
-    ops::report(p.status, kDevBadIndex);
-    q.nq = 0;
-  }
   q.tiles = (q.nq * p.group + rows - 1) / rows;
   q.blocks = (p.own_only ? 0 : (p.prefix_len + 15) / 16) + (q.own + 15) / 16;
   return q;
@@ -193,11 +220,11 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   if (!p.tile_parts) griddep_wait();
 
   // ---- the line: its length, and the run of sequences in which this CTA's part begins
-  const int n_chunks = (p.n_seqs + RUN - 1) / RUN;
+  const int n_seqs = held_seqs(p), n_chunks = (n_seqs + RUN - 1) / RUN;
   long long total = 0;
   for (int c = 0; c < n_chunks; ++c) {
     const int b = c * RUN + threadIdx.x;
-    const Seq q = sequence(p, b, ROWS);
+    const Seq q = sequence(p, n_seqs, b, ROWS);
     if (q.tiles && !q.blocks && b % (int)gridDim.x == (int)blockIdx.x)   // no keys: no part of any warp
       for (long long r = (long long)q.tok0 * p.n_heads; r < (long long)(q.tok0 + q.nq) * p.n_heads; ++r) p.row_parts[r] = make_int2(0, -1);
     long long u = q.units(p.n_kv);
@@ -218,7 +245,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
     long long before = 0;
     int items = 0;
     for (int c = 0; c < n_chunks; ++c) {
-      const Seq q = sequence(p, c * RUN + threadIdx.x, ROWS);
+      const Seq q = sequence(p, n_seqs, c * RUN + threadIdx.x, ROWS);
       long long u = q.units(p.n_kv);
       int it = q.tiles * p.n_kv;
       for (int o = 16; o > 0; o >>= 1) {
@@ -278,7 +305,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   // the sequence that holds unit u, all lanes together
   const auto locate = [&]() {
     while (true) {
-      const Seq x = sequence(p, chunk + lane, ROWS);
+      const Seq x = sequence(p, n_seqs, chunk + lane, ROWS);
       const long long n = x.units(p.n_kv);
       long long incl = n;
       int it = x.tiles * p.n_kv, it_incl = it;
@@ -310,7 +337,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
       before += __shfl_sync(0xffffffffu, incl, 31);
       items += __shfl_sync(0xffffffffu, it_incl, 31);
       chunk += 32;
-      if (chunk >= p.n_seqs) {                 // not reached while the lengths stay what they were
+      if (chunk >= n_seqs) {                   // not reached while the lengths stay what they were
         u1 = u;
         return;
       }
@@ -539,12 +566,16 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
   if (p.tile_parts) griddep_wait();
 }
 
-// Tile `z` of a ragged grid: its sequence and the tile's number in it (warp-wide, all lanes).
-__device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int lane, int& b, int& i) {
+// Tile `z` of the held sequences of a ragged grid: its sequence and the tile's number in it.  `n_seqs`: how
+// many are held, as far as the search came (warp-wide, all lanes).
+__device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int lane, int& b, int& i, int& n_seqs) {
   int before = 0;
-  for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+  n_seqs = p.n_seqs;
+  for (int b0 = 0; b0 < n_seqs; b0 += 32) {
+    const unsigned bad = __ballot_sync(0xffffffffu, b0 + lane < n_seqs && out_of_order(p, b0 + lane));
+    if (bad) n_seqs = b0 + __ffs(bad) - 1;
     int n = 0;
-    if (b0 + lane < p.n_seqs) n = (max(0, p.cu_q[b0 + lane + 1] - p.cu_q[b0 + lane]) * p.group + rows - 1) / rows;
+    if (b0 + lane < n_seqs) n = ((p.cu_q[b0 + lane + 1] - p.cu_q[b0 + lane]) * p.group + rows - 1) / rows;
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -618,6 +649,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   __shared__ float s_row[2][kTile];    // between the two threads of a row
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ volatile int s_held, s_begin, s_end;   // OWN = false: the sequences that are held, their tokens
   volatile int* abort = &s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, split = blockIdx.z;
@@ -650,7 +682,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   int b = 0, ti = blockIdx.x;
   int tok0 = 0, n_rows, own = 0, first_lim = p.prefix_len, last_lim = p.prefix_len;
   if (OWN) {
-    if (!find_tile(p, blockIdx.x, 2 * kTile, lane, b, ti)) {
+    int n_seqs;
+    const bool found = find_tile(p, blockIdx.x, 2 * kTile, lane, b, ti, n_seqs);
+    // the last block finds its tile behind all others, if any: it has seen every offset that counts
+    if (blockIdx.x == gridDim.x - 1 && (threadIdx.x | kvh | split) == 0) tell_held(p, n_seqs);
+    if (!found) {
       if (beside) griddep_wait();
       return;
     }
@@ -659,11 +695,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
     const int cap = p.max_pages * p.page_size, given = p.suffix_lens[b];
     own = max(0, min(given, cap));
     n_rows = min(2 * kTile, nq * p.group - ti * 2 * kTile);
-    if ((given > cap || tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) && threadIdx.x == 0) ops::report(p.status, kDevBadIndex);
-    if (tok0 < 0 || n_rows <= 0 || tok0 + nq > p.n_tokens) {
-      if (beside) griddep_wait();
-      return;
-    }
+    if (given > cap && threadIdx.x == 0) ops::report(p.status, kDevBadIndex);
     first_lim = p.prefix_len + own - nq + 1;
     last_lim = max(0, first_lim + (ti * 2 * kTile + n_rows - 1) / p.group);
   } else {
@@ -676,7 +708,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   const int t0 = split * per, n = max(0, min(n_all, t0 + per) - t0);
   const int n_tiles = n_rows > kTile ? 2 : 1;
 
-  if (warp == 17) tc::tmem_alloc(&s_tmem, 512);
+  if (warp == 17) {
+    tc::tmem_alloc(&s_tmem, 512);
+    if (!OWN) {
+      int n_seqs = p.n_seqs, begin = 0, end = p.n_tokens;
+      if (p.cu_q) {
+        for (int b0 = 0; b0 < n_seqs; b0 += 32) {
+          const unsigned bad = __ballot_sync(0xffffffffu, b0 + lane < n_seqs && out_of_order(p, b0 + lane));
+          if (bad) n_seqs = b0 + __ffs(bad) - 1;
+        }
+        begin = p.cu_q[0];
+        end = p.cu_q[n_seqs];
+        if ((blockIdx.x | kvh | split | lane) == 0) tell_held(p, n_seqs);
+      }
+      if (lane == 0) {
+        s_held = n_seqs;
+        s_begin = begin;
+        s_end = end;
+      }
+    }
+  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
@@ -818,7 +869,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       if (!OWN && p.cu_q) {
         // the row's sequence: where its queries reach into the prefix, they do not see all of it
         const int tok = (row0 + min(lr, n_rows - 1)) / p.group;
-        int lo = 0, hi = p.n_seqs;             // cu_q[lo] <= tok < cu_q[hi], if it is any sequence's
+        int lo = 0, hi = s_held;               // cu_q[lo] <= tok < cu_q[hi], if it is any sequence's
         while (hi - lo > 1) {
           const int mid = (lo + hi) / 2;
           if (p.cu_q[mid] <= tok) lo = mid;
@@ -911,7 +962,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
       if (ok) {
         tc::tc_fence_after();
         const long long tok = tok0 + (row0 + lr) / p.group;
-        const bool live = lr < n_rows && (OWN || !p.cu_q || (tok >= p.cu_q[0] && tok < p.cu_q[p.n_seqs]));
+        const bool live = lr < n_rows && (OWN || (tok >= s_begin && tok < s_end));
         const int head = kvh * p.group + (row0 + lr) % p.group;
         const long long at = (long long)(p.part0 + split) * p.n_tokens * p.n_heads + tok * p.n_heads + head;
         const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -985,11 +1036,13 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Param
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
   const long long tok = row / p.n_heads;
-  if (p.cu_q && (tok < p.cu_q[0] || tok >= p.cu_q[p.n_seqs])) return;   // no sequence's token
+  if (p.cu_q) {
+    const int2 span = __ldcg(p.span);
+    if (tok < span.x || tok >= span.y) return;   // no sequence's token, or a refused one's
+  }
   int2 parts = make_int2(0, -1);
   if (p.rows_run) parts = __ldcg(p.row_parts + row);
   if (parts.y == -2) return;
-  if (parts.x < 0 || parts.y < parts.x || parts.y >= p.row_rows) parts = make_int2(0, -1);   // offsets that the row kernel refused
   const int n_row = parts.y < 0 ? 0 : (parts.y - parts.x) / p.rows_run + 1, n = p.tile_parts + n_row;
   // partial s: the tile kernel's key ranges first
   const auto ml_of = [&](int s) {

@@ -129,6 +129,7 @@ struct Plan {
   int nt;                   // row kernel: tiles of 8 nt rows; 0: not launched
   int row_ctas;
   int64_t tile_rows, row_rows;   // partial rows of each kind
+  bool join;                // there are partials
   int64_t bytes;
 };
 
@@ -207,11 +208,12 @@ int plan_attention(const vx_shared_prefix_args& a, Plan& pl, const Err& e) {
   const long long tile = 8 * pl.nt;
   const long long items = !pl.nt ? 0 : (a.cu_q ? rows / tile + a.n_seqs : a.n_seqs * ((group + tile - 1) / tile)) * c.n_kv_heads;
   const int parts = pl.shared_parts + pl.own_parts;
-  pl.tile_rows = pl.nt || parts > 1 ? (int64_t)parts * a.n_tokens * a.n_heads : 0;
+  pl.join = pl.nt || parts > 1;
+  pl.tile_rows = pl.join ? (int64_t)parts * a.n_tokens * a.n_heads : 0;
   pl.row_rows = pl.nt ? ((int64_t)pl.row_ctas * pattn::row_warps(c.head_dim, pl.nt) + items) * tile : 0;
   if (std::max(pl.shared_pairs, pl.own_pairs) > 0x7fffffff || pl.row_rows > 0x7fffffff || (long long)a.n_tokens * a.n_heads > 0x7fffffff)
     return e.fail(VX_E_RANGE, "%d tokens of %d sequences are too many for one call", a.n_tokens, a.n_seqs);
-  pl.bytes = (pl.tile_rows + pl.row_rows) * (c.head_dim + 2) * 4 + (pl.nt ? (int64_t)a.n_tokens * a.n_heads * 8 : 0);
+  pl.bytes = (pl.tile_rows + pl.row_rows) * (c.head_dim + 2) * 4 + (pl.nt ? (int64_t)a.n_tokens * a.n_heads * 8 : 0) + (pl.join && a.cu_q ? 8 : 0);
   return VX_OK;
 }
 
@@ -380,11 +382,11 @@ extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void*
   p.row_ml = p.tile_ml + pl.tile_rows;
   p.row_parts = (int2*)(p.row_ml + pl.row_rows);
   p.tile_parts = pl.shared_parts + pl.own_parts;
-  p.row_rows = (int)pl.row_rows;
+  p.span = pl.join && a.cu_q ? p.row_parts + (pl.nt ? (int64_t)a.n_tokens * a.n_heads : 0) : nullptr;
   p.rows_run = 8 * pl.nt;
   p.own_only = pl.shared_pairs > 0;
   p.min_blocks = 2;
-  p.direct = !pl.nt && p.tile_parts == 1;
+  p.direct = !pl.join;
   p.n_tokens = a.n_tokens; p.n_seqs = a.n_seqs; p.n_heads = a.n_heads; p.n_kv = c.n_kv_heads; p.group = a.n_heads / c.n_kv_heads;
   p.prefix_len = a.prefix_len; p.page_size = c.page_size; p.n_pages = c.n_pages; p.max_pages = a.max_pages;
   p.scale_log2 = a.scale * pattn::kLog2e;
