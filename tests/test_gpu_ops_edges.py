@@ -7,7 +7,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_ops import BAD_INDEX, BF16, F16, attend_inputs, attend_reference, ints
+from test_gpu_ops import BAD_INDEX, BF16, F16, F32, attend_inputs, attend_reference, check_sample, ints, rand
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -59,3 +59,30 @@ def test_attend_offsets_out_of_order(vx, case):
     off = (out[first:end].double() - want).abs() - tol
     assert held == 0 or float(off.max()) <= 0
     assert bool((out[:first] == 7.0).all()) and bool((out[end:] == 7.0).all())     # no sequence's rows, and refused ones'
+
+
+# ------------------------------------------------------------------------------- sampling
+@pytest.mark.parametrize("temperature", [1.4e-45, 1e-41, 1.2e-38, 1e-37, 1.9e-37, 1e-36, 1e-30, 1e-20])
+@pytest.mark.parametrize("n", [2, 600, 40000])
+def test_sample_lowest_temperatures(vx, temperature, n):
+    """Logits a few temperatures apart, where dividing by so small a number overflows, and far apart."""
+    rng = np.random.default_rng(n)
+    t = float(np.float32(temperature))
+    x = -(rand(6, n, seed=n).abs().double() * 12 * t).float()
+    x[3:5] = -torch.round(rand(2, n, seed=n + 1).abs() * 3) * t                # many equal ones
+    x[5] = rand(1, n, seed=n + 2)[0]
+    x[:, n // 2] = 0.0
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (5, 1.0, 0.0), (0, 0.8, 0.3), (0, 1.0, 1.0), (1000, 0.97, 0.001)):
+        u = rng.random(6) * 0.9999 + 0.00003
+        check_sample(vx, x, u, temperature, k, p, m)
+        by_row = [torch.full((6,), v, device="cuda") for v in (temperature, p, m)]
+        check_sample(vx, x, u, by_row[0], k, by_row[1], by_row[2])
+    check_sample(vx, x.to(BF16), rng.random(6) * 0.9999 + 0.00003, temperature, 0, 0.9, 0.0)
+
+
+def test_sample_low_temperatures_by_row(vx):
+    rng = np.random.default_rng(1)
+    t = torch.tensor([1e-45, 1e-38, 1e-37, 1e-30, 1e-4, 1.0, 0.0, 3e38], device="cuda", dtype=F32)
+    for n in (700, 30000):
+        check_sample(vx, rand(8, n, seed=n), rng.random(8), t, 0, 0.95, 0.0)
+        check_sample(vx, rand(8, n, seed=n) * t[:, None].clamp(max=1.0), rng.random(8), t.clamp(max=1e30), 0, 0.95, 0.0)

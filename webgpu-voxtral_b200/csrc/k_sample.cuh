@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     temp = 1.0;
     k = 1;
   }
-  temp = fmin(fmax(temp, 1e-250), 1e30);       // past these the draw is greedy, or uniform, already
+  temp = fmin(temp, 1e30);                     // uniform by then
   r.mx = mx;
   r.mxd = (double)mx;
   r.c64 = 64.0 * 1.4426950408889634 / temp;
@@ -718,7 +718,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
   const double far = min_p > 0.0 ? fmin(-log2(min_p), (double)kRangeLog2) : (double)kRangeLog2;
   const float span = fmaxf(mx - mn, 1e-30f);                   // bins need not reach past the smallest
   r.cut = fminf((float)(far * to_logit * 1.001 + 1e-6 * to_logit), span);
-  r.scale = (float)(kBins - 1) / r.cut;
+  // finite: below a cut of 6e-36 (temperatures under 2e-37, or any with min-p near 1) the bins are wider
+  // than they need be, which costs an exact pass over more tokens and changes no result
+  r.scale = fminf((float)(kBins - 1) / r.cut, 3.402823466e38f);
   const float sure = fminf((float)(far * to_logit * 0.999), span) * r.scale;
   r.sure = sure < (float)(kBins - 1) ? (int)sure : mx - mn < (float)(far * to_logit * 0.999) ? kBins : kBins - 1;
   const auto reach = [](double share, u64 of) {   // the whole-number mass that `share` of `of` asks for
