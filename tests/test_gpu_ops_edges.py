@@ -61,6 +61,23 @@ def test_attend_offsets_out_of_order(vx, case):
     assert bool((out[:first] == 7.0).all()) and bool((out[end:] == 7.0).all())     # no sequence's rows, and refused ones'
 
 
+@pytest.mark.parametrize("cols", [128, 512, 2048])
+def test_attend_wide_page_tables(vx, cols):
+    """A table as wide as the longest context that a server allows, of which short answers use little: the
+    results, and (the workspace holds a partial for each key range) about as many ranges as with a table
+    cut to length."""
+    lens, prefix = [(1, 1 + 7 * i % 300) for i in range(64)], 32768
+    q, kp, vp, ppages, table, suffix, _ = attend_inputs(lens, prefix, 32, 8, 128, 64, F16, False, seed=cols)
+    wide = torch.full((64, cols), -1, dtype=torch.int32, device="cuda")        # the rest is no page
+    wide[:, :table.shape[1]] = table
+    st = ints([0])
+    got = vx.shared_prefix_attention(q[:64], kp, vp, ppages, prefix, wide, suffix, status=st)
+    want, tol = attend_reference(q[:64], kp, vp, ppages, prefix, table, lens, 128 ** -0.5)
+    assert int(st) == 0 and float(((got.double() - want).abs() - tol).max()) <= 0
+    need = [vx.shared_prefix_attention_workspace(q[:64], kp, vp, ppages, prefix, t, suffix) for t in (table, wide)]
+    assert need[1] >= 0.75 * need[0]
+
+
 # ------------------------------------------------------------------------------- sampling
 @pytest.mark.parametrize("temperature", [1.4e-45, 1e-41, 1.2e-38, 1e-37, 1.9e-37, 1e-36, 1e-30, 1e-20])
 @pytest.mark.parametrize("n", [2, 600, 40000])

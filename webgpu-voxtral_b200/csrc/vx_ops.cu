@@ -137,20 +137,22 @@ struct Plan {
 // key tiles least.  A range's start and end (loading Q, writing the partial) count as four tiles
 // (a tile of 2 x 128 rows takes 2.2 us), and each range's partial is written and read once more.  Where
 // the row kernel runs beside it for `row_us`, the fewest ranges that take half as long leave it the most SMs:
-// 64 sequences past 617 shared keys with 1, 2, 3, 5 ranges 27, 25, 27, 31 us in all.
+// 64 sequences past 617 shared keys with 1, 2, 3, 5 ranges 27, 25, 27, 31 us in all.  row_us goes by what the page
+// tables could hold, so a step with tables of a fixed width would wait for a row kernel that has little to
+// do: fewer ranges may cost the tile kernel kGiveUs at most.
 int tile_parts(long long items, long long tiles, double partial_bytes, double row_us, int sms) {
-  constexpr double kTileUs = 2.2;
+  constexpr double kTileUs = 2.2, kGiveUs = 4.0;
   const double join = 2.0 * partial_bytes / 6e6 / kTileUs;
+  const auto us = [&](int s) {
+    const double waves = (double)((items * s + sms - 1) / sms);
+    return (waves * ((double)((tiles + s - 1) / s) + 4.0) + s * join) * kTileUs;
+  };
   int best = 1;
-  double least = 1e300;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const double waves = (double)((items * s + sms - 1) / sms), cost = waves * ((double)((tiles + s - 1) / s) + 4.0) + s * join;
-    if (cost * kTileUs <= row_us / 2) return s;
-    if (cost < least * 0.999) {
-      least = cost;
-      best = s;
-    }
-  }
+  for (int s = 2; s <= 64 && s <= tiles; ++s)
+    if (us(s) < us(best) * 0.999) best = s;
+  const double most = std::min(row_us / 2, us(best) + kGiveUs);
+  for (int s = 1; s < best; ++s)
+    if (us(s) <= most) return s;
   return best;
 }
 
