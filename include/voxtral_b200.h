@@ -410,7 +410,9 @@ int vx_rope_append_kv(const vx_rope_append_args* a, void* stream, char* err, siz
  * n_heads a multiple of the cache's n_kv_heads; head_dim 64 or 128; page_size 16, 32, 64, 128 or
  * 256; q and out in the cache's type; scale > 0.  Keys that no query token sees may hold any
  * value (NaN too) where they lie past the prefix or past a sequence's keys; keys that some token
- * of a sequence sees must have finite values.  workspace: 256-byte aligned, at least
+ * of a sequence sees must have finite values.  Sums are f32; the weights are rounded to the cache's type
+ * for their product with v (F16: also to 2^-32 of the row's largest, which n keys feel as n 2^-32 of |v|
+ * at most).  workspace: 256-byte aligned, at least
  * vx_shared_prefix_attention_workspace(a) bytes, used by this call alone until it is done. */
 typedef struct vx_shared_prefix_args {
   vx_kv_pages cache;

@@ -78,6 +78,38 @@ def test_attend_wide_page_tables(vx, cols):
     assert need[1] >= 0.75 * need[0]
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("path", ["rows", "shared", "own"])
+@pytest.mark.parametrize("e", [26.0, 26.3])
+def test_attend_long_tails(vx, dtype, path, e):
+    """2^20 equal keys, each at 2^-e of one strong key: by themselves below the steps of an f16 weight,
+    together 1.5 % of the result.  The strong key's value is 0, the others' 1: o = n w / (1 + n w).  The
+    batches are wide enough for each row to take (nearly) all keys in one range, the strong one among them.
+
+    A weight is off by 2^-32 of the largest (f16) and by half a step of its type; a score by (d + 2) 2^-23 of itself, the
+    exponential by 2^-22; the sums of weights and of products, 16 keys at a time, by 2^16 2^-23 each."""
+    n, page, d = 1 << 20, 256, 64
+    kp, vp = torch.zeros((n // page + 1, 1, page, d), dtype=dtype, device="cuda"), torch.ones((n // page + 1, 1, page, d), dtype=dtype, device="cuda")
+    kp[7, 0, 11, 0], vp[7, 0, 11] = 4.0, 0.0
+    pages = torch.arange(n // page + 1, dtype=torch.int32, device="cuda")
+    seqs, each, heads = {"rows": (2072, 1, 1), "shared": (592, 1, 64), "own": (148, 64, 1)}[path]
+    q = torch.zeros((seqs * each, heads, d), dtype=dtype, device="cuda")
+    q[..., 0] = 8.0
+    scale = float(np.float32(e * math.log(2) / 32.0))
+    keys = torch.full((seqs,), n + 1, dtype=torch.int32, device="cuda")
+    if path == "shared":
+        o = vx.shared_prefix_attention(q, kp, vp, pages, n + 1, torch.zeros((seqs, 0), dtype=torch.int32, device="cuda"), keys * 0, scale=scale)
+    else:
+        cu = torch.arange(0, seqs * each + 1, each, dtype=torch.int32, device="cuda") if path == "own" else None
+        o = vx.shared_prefix_attention(q, kp, vp, pages[:0], 0, pages[None].expand(seqs, -1), keys, cu_q=cu, scale=scale)
+    u = torch.finfo(dtype).eps / 2
+    for i in {0, each - 1}:                                                    # query i of each sequence
+        nw = (n - (each - 1 - i)) * math.exp(-32.0 * scale)
+        want = nw / (1 + nw)
+        tol = n * 2.0 ** -32 * (dtype == F16) + want * (2 * u + 2 * (d + 2) * 2.0 ** -23 * 32 * scale + 2 * 2.0 ** -22 + 2 * 2.0 ** -7)
+        assert float((o[i::each].double() - want).abs().max()) <= tol
+
+
 # ------------------------------------------------------------------------------- sampling
 @pytest.mark.parametrize("temperature", [1.4e-45, 1e-41, 1.2e-38, 1e-37, 1.9e-37, 1e-36, 1e-30, 1e-20])
 @pytest.mark.parametrize("n", [2, 600, 40000])

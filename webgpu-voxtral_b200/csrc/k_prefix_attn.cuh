@@ -19,7 +19,10 @@
 // by o = sum_r e^(m_r - m) o_r / sum_r e^(m_r - m) l_r.  Everything but the operands of the
 // matrix products is f32; the weights are rounded to the cache's type for the product with V
 // (half a step of 2^-11 / 2^-8 of a weight, as large as the rounding of V itself and averaged
-// over the keys), their sum l is not.
+// over the keys), their sum l is not.  f16 weights end at 2^-25, which in a long tail adds up: 10^6 equal
+// keys at 2^-26 of one strong key are 1.5 % of its result.  So a row's weights are taken relative to 2^-7
+// (tile kernel, whose reference may lag by 2^8) or 2^-15 (row kernel) of its largest, which uses f16's
+// range to 2^15: a weight is then off by 2^-32 of the largest at most.  The factor cancels against l.
 #pragma once
 #include "vx_ops.cuh"
 #include "vx_tcgen05.cuh"
@@ -101,6 +104,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// Powers of two by which a row's reference lies below its largest score, where its weights may grow to 2^room.
+template <typename T>
+constexpr float below_top(int room) {
+  return sizeof(T) == 2 && ops::Elem<T>::kIdescType == 0 ? 15.f - room : 0.f;   // bf16 has f32's range
 }
 // Barrier of `threads` threads that tells all of them whether one came with `v`.
 __device__ __forceinline__ bool named_bar_or(int id, int threads, bool v) {
@@ -488,7 +496,7 @@ __global__ void __launch_bounds__(row_warps(D, NT) * 32, 1) k_attn_rows(const __
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float m_new = fmaxf(m[n][e], mx);
+        const float m_new = fmaxf(m[n][e], mx - below_top<T>(0));
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
         corr[e] = ex2(m[n][e] - m_use);
         m[n][e] = m_new;
@@ -604,7 +612,7 @@ __device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int 
 // Warps 0-7 and 8-15 each do the softmax of one tile, two threads a row (64 keys each; no shuffles);
 // warp 16 brings the pages in by TMA; one thread of warp 17 issues the products.  While one tile's
 // softmax runs, the other tile's products do.  The reference exponent of a row only moves when its maximum grows
-// by more than 2^8 (weights stay below 2^8, far inside f16's and f32's range), so that O in TMEM is
+// by more than 2^8 (weights stay below 2^8 or, in f16, 2^15, inside f16's and f32's range), so that O in TMEM is
 // hardly ever rescaled.
 //
 // Bound: for a wide batch the tensor cores and the exponentials (a 128 x 128 tile needs 1024 cycles
@@ -902,7 +910,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
           for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
         mx[0] = max3(mx[0], s[K - 4], s[K - 3]);
         mx[1] = max3(mx[1], s[K - 2], s[K - 1]);
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), p.scale_log2, -below_top<T>(8));
         // The two halves' scores are in registers once all have met here, so the weights may take
         // their columns; and all know whether a row of the tile has outgrown its reference
         tc::tc_fence_before();
