@@ -135,3 +135,21 @@ def test_sample_low_temperatures_by_row(vx):
     for n in (700, 30000):
         check_sample(vx, rand(8, n, seed=n), rng.random(8), t, 0, 0.95, 0.0)
         check_sample(vx, rand(8, n, seed=n) * t[:, None].clamp(max=1.0), rng.random(8), t.clamp(max=1e30), 0, 0.95, 0.0)
+
+
+@pytest.mark.parametrize("seqs,heads", [(1, 8), (70, 8), (3, 520)])
+def test_sample_right_behind_the_kernel_that_writes_its_logits(vx, seqs, heads):
+    """Attention lets the next kernel start before it is done; the draw must see what it wrote.  The same
+    buffers again and again with other contents, so that anything old shows."""
+    q, kp, vp, ppages, table, suffix, _ = attend_inputs([(1, 1 + b % 40) for b in range(seqs)], 300, heads, 8, 128, 16, F16, False, seed=seqs)
+    q, u = q[:seqs], torch.full((seqs,), 0.5, dtype=torch.float64, device="cuda")
+    out = torch.empty_like(q)
+    args = [(q * (1 + 0.1 * i)).contiguous() for i in range(8)]
+    got, want = [], []
+    for x in args:
+        vx.shared_prefix_attention(x, kp, vp, ppages, 300, table, suffix, out=out)
+        got.append(vx.sample_logits(out.flatten(1), u, temperature=0.01, top_p=0.9))
+        want.append(out.clone())
+    torch.cuda.synchronize()
+    for g, o in zip(got, want):
+        assert torch.equal(g, vx.sample_logits(o.flatten(1), u, temperature=0.01, top_p=0.9))

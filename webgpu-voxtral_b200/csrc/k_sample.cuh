@@ -355,7 +355,8 @@ __device__ __forceinline__ float clean(float x) {
 }
 // Calls f(x, i) for the logits of the slice, x[0..3] at i (-inf past the end).  Four loads a thread are
 // on their way before the first is used: neither the branches of a ragged end nor what f does to
-// shared memory stand between them.
+// shared memory stand between them.  Ordinary loads: the kernel before may still be writing the logits when
+// this one starts, and the read-only path holds only for what nobody writes while a kernel is there.
 template <typename T, bool FIRST, typename F>
 __device__ __forceinline__ void each_four(const Smem& s, const Slice<T>& sl, F f) {
   constexpr int U = 4, STEP = 4 * kThreads;
@@ -374,7 +375,7 @@ __device__ __forceinline__ void each_four(const Smem& s, const Slice<T>& sl, F f
         typedef typename std::conditional<sizeof(T) == 4, float4, uint2>::type Four;
         Four q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = __ldg(reinterpret_cast<const Four*>(sl.g + i0 + u * STEP));
+        for (int u = 0; u < U; ++u) q[u] = *reinterpret_cast<const Four*>(sl.g + i0 + u * STEP);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if constexpr (sizeof(T) == 4) {
