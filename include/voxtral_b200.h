@@ -361,7 +361,8 @@ int vx_lm_head_argmax_noalloc(const uint16_t* weight, const float* x, int32_t ro
  * nothing did: VX_STATUS_BAD_INDEX, or another code where a bounded wait of a kernel expired (the
  * output is then not valid). */
 #define VX_STATUS_BAD_INDEX 5 /* a page, sequence, offset or length out of range: such a token is
-                                 not written, keys of such a page read as zero */
+                                 not written, keys of such a page read as zero, keys past the end
+                                 of a page table's row are left out */
 
 /* One layer of a paged K/V cache: element (page, head, slot, d) of each pool at
  * page * page_stride + head * head_stride + slot * slot_stride + d.  The engine's own layout

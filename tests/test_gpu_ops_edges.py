@@ -61,6 +61,22 @@ def test_attend_offsets_out_of_order(vx, case):
     assert bool((out[:first] == 7.0).all()) and bool((out[end:] == 7.0).all())     # no sequence's rows, and refused ones'
 
 
+@pytest.mark.parametrize("seqs,each", [(2, 1), (64, 1), (700, 1), (5, 30), (3, 130)])
+@pytest.mark.parametrize("prefix", [90, 2500])
+def test_attend_lengths_past_a_table_of_no_columns(vx, seqs, each, prefix):
+    """Own keys that no page holds are reported and left out, whichever kernels take the prefix."""
+    lens = [(each, 0)] * seqs
+    q, kp, vp, ppages, table, suffix, cu = attend_inputs(lens, prefix, 16, 4, 64, 16, BF16, False, seed=seqs)
+    q, kw = q[:seqs * each], {} if each == 1 else {"cu_q": cu}
+    want, tol = attend_reference(q, kp, vp, ppages, prefix, table, lens, 64 ** -0.5)
+    for bad in (None, seqs - 1, 0):
+        s, st = suffix.clone(), ints([0])
+        if bad is not None:
+            s[bad] = 3
+        got = vx.shared_prefix_attention(q, kp, vp, ppages, prefix, table[:, :0], s, status=st, **kw)
+        assert int(st) == (0 if bad is None else BAD_INDEX)
+        assert float(((got.double() - want).abs() - tol).max()) <= 0
+
 @pytest.mark.parametrize("cols", [128, 512, 2048])
 def test_attend_wide_page_tables(vx, cols):
     """A table as wide as the longest context that a server allows, of which short answers use little: the

@@ -719,6 +719,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attn_tiles(const __grid_con
   if (warp == 17) {
     tc::tmem_alloc(&s_tmem, 512);
     if (!OWN) {
+      if (p.max_pages == 0) {   // no other kernel looks at the lengths: the blocks share them out
+        const long long cta = (long long)blockIdx.x * gridDim.y * gridDim.z + kvh * gridDim.z + split, ctas = (long long)gridDim.x * gridDim.y * gridDim.z;
+        for (long long b = cta * 32 + lane; b < p.n_seqs; b += ctas * 32)
+          if (p.suffix_lens[b] > 0) ops::report(p.status, kDevBadIndex);
+      }
       int n_seqs = p.n_seqs, begin = 0, end = p.n_tokens;
       if (p.cu_q) {
         for (int b0 = 0; b0 < n_seqs; b0 += 32) {
