@@ -1,0 +1,43 @@
+"""The ends of what the serving operators take, on the CPU: gradients and tangents, numbers that do not fit,
+sizes whose sums would not fit 32 bits."""
+import pytest
+
+from test_ops_refusals import F16, P, _append, _attend, _c, _cache, ops  # noqa: F401
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("call,name", [("rope_append_kv", n) for n in ("q", "k", "v", "rope_freq", "k_pages")]
+                         + [("shared_prefix_attention", n) for n in ("q", "k_pages", "v_pages")])
+def test_tangents_are_refused(vx, call, name):
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        a = _append() if call == "rope_append_kv" else _attend()
+        a[name] = fwd.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(vx.VoxtralError, match=f"{name} has a tangent"):
+            getattr(vx, call)(**a)
+        del a[name]
+
+
+@pytest.mark.parametrize("name", ["logits", "u", "temperature", "top_p", "min_p"])
+def test_sample_refuses_tangents_and_gradients(vx, name):
+    import torch.autograd.forward_ad as fwd
+    a = dict(logits=torch.zeros(2, 9), u=torch.zeros(2, dtype=torch.float64), temperature=torch.ones(2), top_p=torch.ones(2), min_p=torch.ones(2))
+    with fwd.dual_level():
+        b = dict(a)
+        b[name] = fwd.make_dual(a[name], torch.ones_like(a[name]))
+        with pytest.raises(vx.VoxtralError, match="has a tangent"):
+            vx.sample_logits(b.pop("logits"), b.pop("u"), **b)
+    a[name] = a[name].clone().requires_grad_()
+    with pytest.raises(vx.VoxtralError, match="requires a gradient"):
+        vx.sample_logits(a["logits"], a["u"], **{k: v for k, v in a.items() if k not in ("logits", "u")})
+    with torch.no_grad(), pytest.raises(vx.VoxtralError, match="CUDA device"):
+        vx.sample_logits(a["logits"], a["u"], **{k: v for k, v in a.items() if k not in ("logits", "u")})
+
+
+def test_append_refuses_gradients_of_frequencies(vx):
+    freq = torch.zeros(32, requires_grad=True)
+    with pytest.raises(vx.VoxtralError, match="rope_freq requires a gradient"):
+        vx.rope_append_kv(**_append(rope_freq=freq))
+    with torch.no_grad(), pytest.raises(vx.VoxtralError, match="CUDA device"):
+        vx.rope_append_kv(**_append(rope_freq=freq))

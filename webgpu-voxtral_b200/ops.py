@@ -25,6 +25,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from .engine import VX_OK, VoxtralError, load_library
 
@@ -93,6 +94,17 @@ def _rows(name, t, dims, dtypes):
     return shape, stride
 
 
+def _no_gradient(names: str, *tensors):
+    """Refuses tangents, and gradients of what _rows has not looked at: the operators compute neither."""
+    for i, t in enumerate(tensors):
+        if t is None or not t.is_floating_point():
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{names.split()[i]} requires a gradient, which this operator does not compute")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f"{names.split()[i]} has a tangent, which this operator does not carry on")
+
+
 def _vector(name, t, dtype, n=None):
     shape = t.shape
     if len(shape) != 1 or t.dtype is not dtype or not t.is_contiguous():
@@ -148,6 +160,8 @@ def rope_append_kv(q, k, v, k_pages, v_pages, page_table, seq_ids, positions, ro
     if rope_positions is not None:
         _vector("rope_positions", rope_positions, _INT, n)
     _vector("rope_freq", rope_freq, torch.float32)
+    if rope_freq.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient("k v q rope_freq k_pages v_pages q_out", k, v, q, rope_freq, k_pages, v_pages, q_out)
     heads = q_ptr = out_ptr = 0
     qs = os = (0, 0)
     if q is not None:
@@ -232,6 +246,8 @@ def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suff
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_pages.shape[0]} pages of {cache[10]}")
     if cu_q is not None:
         _vector("cu_q", cu_q, _INT, seqs + 1)
+    if forward_ad._current_level >= 0:
+        _no_gradient("q k_pages v_pages out", q, k_pages, v_pages, out)
     device = q.get_device()
     if not (0 <= device == k_pages.get_device() == v_pages.get_device() == prefix_pages.get_device() == page_table.get_device()
             == suffix_lens.get_device() == out.get_device() and (cu_q is None or cu_q.get_device() == device)
@@ -276,6 +292,8 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
                         f"not {v.dtype} {tuple(v.shape)}")
             tensors.append(v)
             each[i], one[i] = v.data_ptr(), 0
+    if forward_ad._current_level >= 0 or any(t.requires_grad for t in tensors):
+        _no_gradient("logits u setting setting setting", logits, u, *tensors[2:])
     if not -2**31 <= one[3] < 2**31:
         _refuse(f"top_k {one[3]} does not fit 32 bits")
     if out is None:
