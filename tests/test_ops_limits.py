@@ -41,3 +41,18 @@ def test_append_refuses_gradients_of_frequencies(vx):
         vx.rope_append_kv(**_append(rope_freq=freq))
     with torch.no_grad(), pytest.raises(vx.VoxtralError, match="CUDA device"):
         vx.rope_append_kv(**_append(rope_freq=freq))
+
+
+@pytest.mark.parametrize("kw,word", [(dict(top_k=2.5), "top_k 2.5"), (dict(top_k=float("nan")), "top_k nan"), (dict(top_k=None), "top_k None"),
+                                     (dict(top_k=2**31), "32 bits"), (dict(temperature="warm"), "temperature warm"),
+                                     (dict(min_p=None), "min_p None"), (dict(top_p=10**400), "top_p 1000"), (dict(top_k=50.0), "CUDA device")])
+def test_sample_refuses_numbers(vx, kw, word):
+    with pytest.raises(vx.VoxtralError, match=word):
+        vx.sample_logits(torch.zeros(2, 9), torch.zeros(2, dtype=torch.float64), **kw)
+
+
+@pytest.mark.parametrize("value,word", [(30.5, "prefix_len 30.5"), (None, "prefix_len None"), (2**31, "prefix_len 2147483648"),
+                                        (float("inf"), "prefix_len inf"), (30.0, "CUDA device"), (torch.tensor(30), "CUDA device")])
+def test_attend_refuses_prefix_lengths(vx, value, word):
+    with pytest.raises(vx.VoxtralError, match=word):
+        vx.shared_prefix_attention(**_attend(prefix_len=value))

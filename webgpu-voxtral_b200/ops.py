@@ -105,6 +105,24 @@ def _no_gradient(names: str, *tensors):
             _refuse(f"{names.split()[i]} has a tangent, which this operator does not carry on")
 
 
+def _whole(name, v):
+    """A whole number that fits 32 bits."""
+    try:
+        n = int(v)
+        if n == v and -2**31 <= n < 2**31:
+            return n
+    except (TypeError, ValueError, OverflowError):
+        pass
+    _refuse(f"{name} {v} must be a whole number of 32 bits")
+
+
+def _real(name, v):
+    try:
+        return float(v)
+    except (TypeError, ValueError, OverflowError):
+        _refuse(f"{name} {v} must be a number")
+
+
 def _vector(name, t, dtype, n=None):
     shape = t.shape
     if len(shape) != 1 or t.dtype is not dtype or not t.is_contiguous():
@@ -214,7 +232,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
         workspace = q.new_empty(need >> 1)       # 2-byte elements; need is a multiple of 4
         ptr, held = workspace.data_ptr(), need
     _call(_library().vx_shared_prefix_attention,
-          _PREFIX.pack(*cache, *pointers[:11], ptr, held, pointers[11], *sizes[6:], 1.0 / math.sqrt(sizes[3]) if scale is None else scale),
+          _PREFIX.pack(*cache, *pointers[:11], ptr, held, pointers[11], *sizes[6:], 1.0 / math.sqrt(sizes[3]) if scale is None else _real("scale", scale)),
           device)
     return out
 
@@ -242,6 +260,7 @@ def _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suff
     seqs, pages, table_stride = _table(page_table)
     _vector("suffix_lens", suffix_lens, _INT, seqs)
     _vector("prefix_pages", prefix_pages, _INT)
+    prefix_len = _whole("prefix_len", prefix_len)
     if prefix_len < 0 or prefix_pages.shape[0] * cache[10] < prefix_len:
         _refuse(f"prefix_len {prefix_len} does not fit {prefix_pages.shape[0]} pages of {cache[10]}")
     if cu_q is not None:
@@ -294,8 +313,10 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             each[i], one[i] = v.data_ptr(), 0
     if forward_ad._current_level >= 0 or any(t.requires_grad for t in tensors):
         _no_gradient("logits u setting setting setting", logits, u, *tensors[2:])
-    if not -2**31 <= one[3] < 2**31:
-        _refuse(f"top_k {one[3]} does not fit 32 bits")
+    for i in range(3):
+        if type(one[i]) is not float:
+            one[i] = _real(("temperature", "top_p", "min_p")[i], one[i])
+    one[3] = _whole("top_k", one[3])
     if out is None:
         out = torch.empty(rows, dtype=_INT, device=logits.device)
     else:
@@ -305,6 +326,6 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     if device < 0 or any(t.get_device() != device for t in tensors):
         _misplaced("logits u setting setting setting setting out", *tensors)
     _call(_library().vx_sample_logits,
-          _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), stride[0], one[0], one[1], one[2], int(one[3]),
+          _SAMPLE.pack(logits.data_ptr(), u.data_ptr(), *each, out.data_ptr(), stride[0], one[0], one[1], one[2], one[3],
                        _DTYPE[logits.dtype], rows, cols, 0), device)
     return out
