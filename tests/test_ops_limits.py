@@ -56,3 +56,16 @@ def test_sample_refuses_numbers(vx, kw, word):
 def test_attend_refuses_prefix_lengths(vx, value, word):
     with pytest.raises(vx.VoxtralError, match=word):
         vx.shared_prefix_attention(**_attend(prefix_len=value))
+
+
+@pytest.mark.parametrize("prefix,pages,code,word", [(2**30, 2**26, -4, "together"), (2**30, 2**26 - 15, -4, "together"),
+                                                    (2**30, 2**26 - 16, -2, "CUDA"), (1, 2**26, -2, "CUDA")])
+def test_attend_positions_fit_32_bits(ops, prefix, pages, code, word):
+    """2^30 prefix keys and 2^30 own ones have a last position that no int holds (pages may repeat, so no
+    such memory is needed).  The calls that fit get as far as looking for a device."""
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses")
+    a = dict(q=P, out=2 * P, qs=256, qh=64, os=256, oh=64, ppages=P, table=P, suffix=P, cu=0, status=0, ws=0, wsb=0, tstride=1, n_tokens=2, seqs=2,
+             heads=4, prefix=prefix, pages=pages, scale=0.125)
+    rc, msg = _c(ops, "vx_shared_prefix_attention", ops._PREFIX.pack(*_cache(), *a.values()))
+    assert rc == code and word in msg, (rc, msg)

@@ -168,6 +168,9 @@ int check_attention(const vx_shared_prefix_args& a, const Err& e) {
     return e.fail(VX_E_RANGE, "n_heads %d is not a multiple of n_kv_heads %d", a.n_heads, c.n_kv_heads);
   if (a.prefix_len < 0 || a.prefix_len > (1 << 30) || a.max_pages < 0 || (int64_t)a.max_pages * c.page_size > (1 << 30))
     return e.fail(VX_E_RANGE, "prefix_len %d, %d pages of %d own keys: at most 2^30 each", a.prefix_len, a.max_pages, c.page_size);
+  // positions and limits are ints, up to a tile past the last key
+  if ((int64_t)a.prefix_len + (int64_t)a.max_pages * c.page_size > 0x7fffff00)
+    return e.fail(VX_E_RANGE, "prefix_len %d and %d pages of %d own keys: less than 2^31 - 256 together", a.prefix_len, a.max_pages, c.page_size);
   if (!(a.scale > 0.f) || a.scale > 1e30f) return e.fail(VX_E_RANGE, "scale %g must be positive", (double)a.scale);
   if (!a.cu_q && a.n_tokens != a.n_seqs)
     return e.fail(VX_E_INVALID, "%d tokens for %d sequences: cu_q is needed", a.n_tokens, a.n_seqs);
