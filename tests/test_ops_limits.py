@@ -69,3 +69,11 @@ def test_attend_positions_fit_32_bits(ops, prefix, pages, code, word):
              heads=4, prefix=prefix, pages=pages, scale=0.125)
     rc, msg = _c(ops, "vx_shared_prefix_attention", ops._PREFIX.pack(*_cache(), *a.values()))
     assert rc == code and word in msg, (rc, msg)
+
+
+def test_attend_refuses_its_queries_as_output(ops):
+    """Some rows' results would be written while other warps still read their queries."""
+    a = dict(q=P, out=P, qs=256, qh=64, os=256, oh=64, ppages=P, table=P, suffix=P, cu=0, status=0, ws=0, wsb=0, tstride=1, n_tokens=2, seqs=2,
+             heads=4, prefix=30, pages=1, scale=0.125)
+    rc, msg = _c(ops, "vx_shared_prefix_attention", ops._PREFIX.pack(*_cache(), *a.values()))
+    assert rc == -1 and "overlap" in msg, (rc, msg)

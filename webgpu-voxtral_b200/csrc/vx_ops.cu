@@ -368,6 +368,7 @@ extern "C" int vx_shared_prefix_attention(const vx_shared_prefix_args* ap, void*
   if (!aligned(a.q) || !aligned(a.out) || !row_strides(0, a.q_token_stride, a.q_head_stride) ||
       !row_strides(0, a.out_token_stride, a.out_head_stride))
     return e.fail(VX_E_INVALID, "rows of q and out must start on 16-byte boundaries");
+  if (a.out == a.q) return e.fail(VX_E_INVALID, "out must not overlap q");
   Plan pl{};
   rc = plan_attention(a, pl, e);
   if (rc) return rc;

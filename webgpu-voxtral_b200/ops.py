@@ -218,7 +218,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_pages, prefix_len: int, 
     int32) and suffix_lens[b] keys of its own (row b of page_table), those of its query tokens among
     them; its query tokens are rows cu_q[b]:cu_q[b + 1] (int32, n_seqs + 1 of them), without cu_q
     row b.  The last query token sees every key of its sequence, each one before it one key less.
-    scale defaults to 1 / sqrt(head_dim).  Returns out, shaped as q; rows past cu_q's last are not
+    scale defaults to 1 / sqrt(head_dim).  Returns out, shaped as q, of which it must share no memory; rows past cu_q's last are not
     written, a row that sees no key is 0.  workspace: a uint8 tensor of at least
     shared_prefix_attention_workspace bytes that no other call uses at the same time."""
     cache, sizes, pointers, device, out = _prefix_args(q, k_pages, v_pages, prefix_pages, prefix_len, page_table, suffix_lens, cu_q, out, status)
