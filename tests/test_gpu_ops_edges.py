@@ -126,6 +126,47 @@ def test_attend_long_tails(vx, dtype, path, e):
         assert float((o[i::each].double() - want).abs().max()) <= tol
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("each,own,prefix", [(1, 37, 700), (1, 90, 0), (70, 130, 0), (20, 33, 3000)])
+def test_append_and_attend_in_one_layer_of_a_cache(vx, dtype, each, own, prefix):
+    """K and V as views of one allocation [page][layer][K or V][head][slot][64]: pages lie far apart, and all
+    other layers stay as they are."""
+    seqs, heads, kv, d, page, layers, layer = 4, 8, 2, 64, 16, 3, 1
+    shared, held = -(-prefix // page), -(-own // page)
+    order = np.random.default_rng(own).permutation(shared + seqs * held + 2).astype(np.int32)
+    buf = torch.full((len(order), layers, 2, kv, page, d), math.nan, dtype=dtype, device="cuda")
+    kp, vp = buf[:, layer, 0], buf[:, layer, 1]
+    ppages = torch.from_numpy(order[:shared]).cuda()
+    table = torch.from_numpy(order[shared:shared + seqs * held].reshape(seqs, held)).cuda()
+    # every key of the prefix and of the sequences goes in through the append, its rotation left out
+    k, v = rand(prefix + seqs * own, kv, d, dtype=dtype, seed=1), rand(prefix + seqs * own, kv, d, dtype=dtype, seed=2)
+    rows = [[0] * prefix, [b for b in range(seqs) for _ in range(own)]]
+    where = [list(range(prefix)), list(range(own)) * seqs]
+    for at, tab, seq, pos in ((0, ppages[None], rows[0], where[0]), (prefix, table, rows[1], where[1])):
+        st = ints([0])
+        vx.rope_append_kv(None, k[at:at + len(seq)], v[at:at + len(seq)], kp, vp, tab, ints(seq), ints(pos),
+                          torch.zeros(0, device="cuda"), status=st)
+        assert int(st) == 0
+    assert torch.equal(kp[order[shared], :, 0], k[prefix])
+    lens = [(each, own)] * seqs
+    q = rand(seqs * each, heads, d, dtype=dtype, seed=3)
+    kw = {} if each == 1 else {"cu_q": ints([each * b for b in range(seqs + 1)])}
+    got = vx.shared_prefix_attention(q, kp, vp, ppages, prefix, table, ints([own] * seqs), **kw)
+    want, tol = attend_reference(q, kp, vp, ppages, prefix, table, lens, d ** -0.5)
+    assert float(((got.double() - want).abs() - tol).max()) <= 0
+    buf[:, layer] = math.nan
+    assert bool(torch.isnan(buf).all())
+
+
+def test_attend_one_chunk_among_single_tokens(vx):
+    lens = [(512, 600)] + [(1, 1 + 17 * b % 300) for b in range(40)]
+    for prefix, dtype in ((0, F16), (1500, BF16)):
+        q, kp, vp, ppages, table, suffix, cu = attend_inputs(lens, prefix, 16, 4, 64, 16, dtype, False, seed=prefix)
+        got = vx.shared_prefix_attention(q[:552], kp, vp, ppages, prefix, table, suffix, cu_q=cu)
+        want, tol = attend_reference(q[:552], kp, vp, ppages, prefix, table, lens, 64 ** -0.5)
+        assert float(((got.double() - want).abs() - tol).max()) <= 0
+
+
 # ------------------------------------------------------------------------------- sampling
 @pytest.mark.parametrize("temperature", [1.4e-45, 1e-41, 1.2e-38, 1e-37, 1.9e-37, 1e-36, 1e-30, 1e-20])
 @pytest.mark.parametrize("n", [2, 600, 40000])
