@@ -167,6 +167,18 @@ def test_attend_one_chunk_among_single_tokens(vx):
         assert float(((got.double() - want).abs() - tol).max()) <= 0
 
 
+@pytest.mark.parametrize("seqs,prefix,each", [(3, 50, 1), (64, 2000, 1), (3, 200, 90)])
+def test_attend_over_broadcast_heads(vx, seqs, prefix, each):
+    """One K/V head expanded to four (a head stride of 0) gives what four copies of it give."""
+    lens = [(each, each + 9 * b % 70) for b in range(seqs)]
+    q, kp, vp, ppages, table, suffix, cu = attend_inputs(lens, prefix, 8, 1, 64, 16, F16, False, seed=seqs)
+    q, kw = q[:seqs * each], {} if each == 1 else {"cu_q": cu}
+    wide = [x.expand(-1, 4, -1, -1) for x in (kp, vp)]
+    got = vx.shared_prefix_attention(q, *wide, ppages, prefix, table, suffix, **kw)
+    want = vx.shared_prefix_attention(q, *(x.contiguous() for x in wide), ppages, prefix, table, suffix, **kw)
+    assert torch.equal(got, want)
+
+
 # ------------------------------------------------------------------------------- sampling
 @pytest.mark.parametrize("temperature", [1.4e-45, 1e-41, 1.2e-38, 1e-37, 1.9e-37, 1e-36, 1e-30, 1e-20])
 @pytest.mark.parametrize("n", [2, 600, 40000])
