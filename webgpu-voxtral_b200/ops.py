@@ -301,7 +301,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     rows, cols = shape
     if u.dtype is not torch.float64 or u.shape != (rows,) or not u.is_contiguous():
         _refuse(f"u must be a contiguous float64 tensor of {rows} elements, not {u.dtype} {tuple(u.shape)}")
-    tensors, each, one = [logits, u], [0, 0, 0, 0], [temperature, top_p, min_p, top_k]
+    tensors, each, one, graded = [logits, u], [0, 0, 0, 0], [temperature, top_p, min_p, top_k], u.requires_grad
     for i in range(4):
         v = one[i]
         if isinstance(v, torch.Tensor):
@@ -310,13 +310,14 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
                 _refuse(f"{('temperature', 'top_p', 'min_p', 'top_k')[i]} must be a number or a contiguous {kind} tensor of {rows} elements, "
                         f"not {v.dtype} {tuple(v.shape)}")
             tensors.append(v)
+            graded = graded or v.requires_grad
             each[i], one[i] = v.data_ptr(), 0
-    if forward_ad._current_level >= 0 or any(t.requires_grad for t in tensors):
-        _no_gradient("logits u setting setting setting", logits, u, *tensors[2:])
-    for i in range(3):
-        if type(one[i]) is not float:
-            one[i] = _real(("temperature", "top_p", "min_p")[i], one[i])
-    one[3] = _whole("top_k", one[3])
+        elif type(v) is not (float if i < 3 else int):
+            one[i] = _real(("temperature", "top_p", "min_p")[i], v) if i < 3 else _whole("top_k", v)
+    if graded or forward_ad._current_level >= 0:
+        _no_gradient("logits u setting setting setting setting", logits, u, *tensors[2:])
+    if not -2**31 <= one[3] < 2**31:
+        _refuse(f"top_k {one[3]} must be a whole number of 32 bits")
     if out is None:
         out = torch.empty(rows, dtype=_INT, device=logits.device)
     else:
