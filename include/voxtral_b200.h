@@ -365,8 +365,9 @@ int vx_lm_head_argmax_noalloc(const uint16_t* weight, const float* x, int32_t ro
                                  of a page table's row are left out */
 
 /* One layer of a paged K/V cache: element (page, head, slot, d) of each pool at
- * page * page_stride + head * head_stride + slot * slot_stride + d.  The engine's own layout
- * ([page][layer][K|V][head][64][128]) is such a pool, and so is a token-major one. */
+ * page * page_stride + head * head_stride + slot * slot_stride + d.  A cache laid out
+ * as the engine's own ([page][layer][K|V][head][64][128]) holds such a pool for each layer, and a
+ * token-major one is such a pool; the engine hands out no pointers to its own. */
 typedef struct vx_kv_pages {
   void *k, *v;
   int64_t k_page_stride, k_head_stride, k_slot_stride;
@@ -409,7 +410,8 @@ int vx_rope_append_kv(const vx_rope_append_args* a, void* stream, char* err, siz
  * breaks that is refused with all after it (VX_STATUS_BAD_INDEX, their rows are not written).
  * A negative length counts as 0.  out must not overlap q or the cache.
  * n_heads a multiple of the cache's n_kv_heads; head_dim 64 or 128; page_size 16, 32, 64, 128 or
- * 256; q and out in the cache's type; scale > 0.  Keys that no query token sees may hold any
+ * 256; q and out in the cache's type; scale > 0; prefix_len and max_pages * page_size at most 2^30 each and
+ * 2^31 - 256 together.  Keys that no query token sees may hold any
  * value (NaN too) where they lie past the prefix or past a sequence's keys; keys that some token
  * of a sequence sees must have finite values.  Sums are f32; the weights are rounded to the cache's type
  * for their product with v (F16: also to 2^-32 of the row's largest, which n keys feel as n 2^-32 of |v|
@@ -435,7 +437,8 @@ int vx_shared_prefix_attention(const vx_shared_prefix_args* a, void* stream, cha
  * likely token has w = 1), top_k keeps the first k (0 or less: all), top_p the shortest run whose
  * mass reaches top_p of what is left (1 or more: all; at least one token); the token is the
  * first whose running mass reaches u * (kept mass), u in [0, 1).  With top_k 0 and min_p 0 this is
- * the order and rule of sampleTopP (src/engine.ts:247-289), masses in f64.  temperature <= 0: the
+ * the order and rule of sampleTopP (src/engine.ts:247-289), masses in f64, with settings that are f32
+ * (0.9 counts as 0.89999998; vx_set_sampling keeps doubles).  temperature <= 0: the
  * first of the largest (values above 1e30 count as 1e30).  out[r]: the index, -1 for a row without
  * a finite or +inf logit (NaN counts as -inf; where there is +inf, those tokens alone are drawn).
  * Each setting is a device array by row, or (array null) the value beside it for all rows, with

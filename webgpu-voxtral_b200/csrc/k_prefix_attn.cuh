@@ -12,11 +12,12 @@
 // query token a sequence it takes the rows of all sequences through the shared prefix, which is
 // so read and multiplied once for the batch.  The row kernel takes up to 32 rows of one sequence
 // through their keys at the rate of memory.  Which of them run, and on which keys, is plan_attention's choice
-// (vx_ops.cu).  One B200: 64 sequences of 32 heads on 8 K/V heads of 128 past 32768 shared keys 62 us (the
-// prefix alone 50 us: 690 TFLOP/s, 134 MB read once), past 617 shared and 1 to 1500 own keys 25 us.
+// (vx_ops.cu).  One B200, in a captured graph: 64 sequences of 32 heads on 8 K/V heads of 128 past 32768 shared
+// keys 63 us (the prefix alone 49 us: 700 TFLOP/s, 134 MB read once), past 617 shared and 1 to 1500 own
+// keys 25 us.
 //
 // Softmax splits over ranges of keys: a range leaves (m, l, o) of its own keys, and ranges join
-// by o = sum_r e^(m_r - m) o_r / sum_r e^(m_r - m) l_r.  Everything but the operands of the
+// by o = sum_r e^(m_r - m) o_r / sum_r e^(m_r - m) l_r (online softmax, Milakov and Gimelshein 2018).  Everything but the operands of the
 // matrix products is f32; the weights are rounded to the cache's type for the product with V
 // (half a step of 2^-11 / 2^-8 of a weight, as large as the rounding of V itself and averaged
 // over the keys), their sum l is not.  f16 weights end at 2^-25, which in a long tail adds up: 10^6 equal
@@ -613,10 +614,11 @@ __device__ __forceinline__ bool find_tile(const Params& p, int z, int rows, int 
 // warp 16 brings the pages in by TMA; one thread of warp 17 issues the products.  While one tile's
 // softmax runs, the other tile's products do.  The reference exponent of a row only moves when its maximum grows
 // by more than 2^8 (weights stay below 2^8 or, in f16, 2^15, inside f16's and f32's range), so that O in TMEM is
-// hardly ever rescaled.
+// hardly ever rescaled.  (Both, the two tiles in turns and the reference that lags, are published
+// techniques for attention on these tensor cores.)
 //
 // Bound: for a wide batch the tensor cores and the exponentials (a 128 x 128 tile needs 1024 cycles
-// of products at head_dim 128 and 1024 of ex2), for a narrow one the reading of K and V.
+// of products at head_dim 128, 512 at 64, and 1024 of ex2), for a narrow one the reading of K and V.
 constexpr int kTile = 128;
 constexpr int kTileThreads = 576;   // 16 warps of softmax, one that loads, one that multiplies
 template <int D>

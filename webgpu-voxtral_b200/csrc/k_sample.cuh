@@ -27,7 +27,7 @@
 //
 // Bound: not HBM (200 rows of 131072 f32 logits would take 16 us) but the pass of the masses, about
 // 45 instructions and two or three shared-memory atomics a logit.  One B200: those 200 rows 143 us
-// with top-p 0.95, 67 us with top-k 50; 64 rows of 131072 bf16 logits with all filters 35 us.
+// with top-p 0.95, 67 us with top-k 50; 64 rows of 131072 bf16 logits with all filters 34 us (in a captured graph).
 #pragma once
 #include <cooperative_groups.h>
 

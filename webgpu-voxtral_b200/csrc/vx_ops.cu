@@ -137,9 +137,10 @@ struct Plan {
 // key tiles least.  A range's start and end (loading Q, writing the partial) count as four tiles
 // (a tile of 2 x 128 rows takes 2.2 us), and each range's partial is written and read once more.  Where
 // the row kernel runs beside it for `row_us`, the fewest ranges that take half as long leave it the most SMs:
-// 64 sequences past 617 shared keys with 1, 2, 3, 5 ranges 27, 25, 27, 31 us in all.  row_us goes by what the page
+// 64 sequences past 617 shared and 1 to 1500 own keys with 1, 2, 3, 5 ranges 25, 25, 27, 30 us in all.  row_us goes by what the page
 // tables could hold, so a step with tables of a fixed width would wait for a row kernel that has little to
-// do: fewer ranges may cost the tile kernel kGiveUs at most.
+// do: fewer ranges may cost the tile kernel kGiveUs at most (64 sequences past 32768 shared keys: tables of 320,
+// 8192, 32768, 131072 own keys 69, 71, 71, 71 us; by row_us alone 69, 87, 278, 539).
 int tile_parts(long long items, long long tiles, double partial_bytes, double row_us, int sms) {
   constexpr double kTileUs = 2.2, kGiveUs = 4.0;
   const double join = 2.0 * partial_bytes / 6e6 / kTileUs;
@@ -170,7 +171,7 @@ int check_attention(const vx_shared_prefix_args& a, const Err& e) {
     return e.fail(VX_E_RANGE, "prefix_len %d, %d pages of %d own keys: at most 2^30 each", a.prefix_len, a.max_pages, c.page_size);
   // positions and limits are ints, up to a tile past the last key
   if ((int64_t)a.prefix_len + (int64_t)a.max_pages * c.page_size > 0x7fffff00)
-    return e.fail(VX_E_RANGE, "prefix_len %d and %d pages of %d own keys: less than 2^31 - 256 together", a.prefix_len, a.max_pages, c.page_size);
+    return e.fail(VX_E_RANGE, "prefix_len %d and %d pages of %d own keys: at most 2^31 - 256 together", a.prefix_len, a.max_pages, c.page_size);
   if (!(a.scale > 0.f) || a.scale > 1e30f) return e.fail(VX_E_RANGE, "scale %g must be positive", (double)a.scale);
   if (!a.cu_q && a.n_tokens != a.n_seqs)
     return e.fail(VX_E_INVALID, "%d tokens for %d sequences: cu_q is needed", a.n_tokens, a.n_seqs);
@@ -423,8 +424,8 @@ extern "C" int vx_sample_logits(const vx_sample_args* ap, void* stream, char* er
   if (!sms) return e.fail(VX_E_CUDA, "no current CUDA device");
   // CTAs a row: more of them while all rows together give an SM less than one and a half (two fit),
   // none with fewer than 16384 logits.  One B200: 64 rows of 131072 bf16 logits with 2, 4, 8 CTAs a row
-  // 47, 35, 43 us; 200 rows of f32 with 1, 2, 4 158, 143, 162 us; one row with 1, 4, 8 95, 36, 26 us; 64
-  // rows of 8320 with 1, 2 CTAs 10, 12 us
+  // 47, 34, 43 us; 200 rows of f32 with 1, 2, 4 159, 142, 160 us; one row with 1, 4, 8 92, 34, 23 us; 64
+  // rows of 8320 with 1, 2 CTAs 10, 12 us (top-k 64), 23, 26 us (top-p alone)
   int cluster = 1;
   while (cluster < sample::kMaxCluster && 2ll * a.n_rows * cluster < 3ll * sms && a.n_cols > 16384 * cluster) cluster *= 2;
   if ((long long)a.n_rows * cluster > 0x7fffffff) return e.fail(VX_E_RANGE, "%d rows are too many for one call", a.n_rows);
